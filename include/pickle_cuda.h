@@ -398,6 +398,108 @@ PICKLE_CUDA_API int  pickle_cuda_generate_sampled(pickle_cuda_model_t* m, const 
                                                   int n_gen, int eos_id, float temp, float top_p, uint32_t seed,
                                                   int32_t* out_ids, int* n_out, float* last_logits, size_t* kv_pos);
 
+/* ---- Paged KV cache, BF16 or 8-bit rows ----
+ * No counterpart in the reference, whose cache is one F32 array per
+ * conversation. A pool of pages of page_size positions is shared by any
+ * number of sequences; a page table names the pages of each. All calls are
+ * stateless, asynchronous on `stream` and use the current device; every
+ * buffer belongs to the caller.
+ *
+ * Pool: uint8 [n_pages][n_kv_heads][page_size / 16][cell]. A cell holds 16
+ * positions of one KV head, so that a run of positions of one head is one
+ * contiguous byte range holding everything its reader needs:
+ *     K rows [16][D], V rows [16][D], K scales [16][D/32], V scales [16][D/32]
+ * (BF16 rows: 2 bytes an element, no scales; a cell is 64 D bytes. 8-bit
+ * rows: one byte an element; a cell is 33 D bytes). An 8-bit element is
+ * code * 2^(scale - 127), code an int8 or an E4M3 number; a scale byte
+ * covers 32 consecutive elements of a row and is the smallest power of two
+ * for which every code is in range without clipping (2^-111 at least, so
+ * blocks below about 2^-105 lose precision). A power of two makes every
+ * element exactly a BF16 number: the tensor cores multiply the values the
+ * cache stands for. A block with an element that is not finite gets scale
+ * 255 and codes 0 and reads back as NaN. */
+#define PICKLE_CUDA_KV_BF16 0
+#define PICKLE_CUDA_KV_I8   1
+#define PICKLE_CUDA_KV_E4M3 2
+/* Element type of q, k, v, output rows. */
+#define PICKLE_CUDA_ROW_F32  0
+#define PICKLE_CUDA_ROW_BF16 1
+
+typedef struct {
+    void* pool;         /* device, 16-byte aligned; pickle_cuda_pages_bytes(...) bytes */
+    int   kv_type;      /* PICKLE_CUDA_KV_* */
+    int   n_pages;
+    int   page_size;    /* positions per page, a multiple of 16 */
+    int   n_kv_heads;   /* HK */
+    int   head_dim;     /* D: 64 or 128 */
+    int*  err;          /* device error word (0 = none) or NULL: 5 = a kv_len above max_kv, more than max_q
+                           rows of one sequence, a page id outside the pool, a position past the RoPE
+                           table; other codes = a bounded wait that gave up */
+} pickle_cuda_pages_t;
+
+/* The sequences of one call. Sequence b has the rows
+ * [q_start[b], q_start[b+1]) of the call's q / k / v / output (q_start NULL:
+ * one row each, row b); row i of its n rows is position
+ * kv_len[b] - n + i, so kv_len counts the call's own tokens. Position p
+ * lies in page table[b * table_stride + p / page_size]. A row at a negative
+ * position (an unused entry of a padded batch: kv_len 0) touches no page
+ * and gets zeros. Rows from q_start[n_seqs] on are left as they were. All arrays are
+ * device memory and are read when the kernels run, so a captured graph
+ * follows them. */
+typedef struct {
+    int        n_seqs;
+    int        n_tok;        /* rows of the call's buffers */
+    int        max_q;        /* no sequence has more rows in this call */
+    int        max_kv;       /* no kv_len is larger; <= table_stride * page_size */
+    const int* q_start;      /* [n_seqs + 1], ascending from 0, or NULL (then max_q = 1, n_tok = n_seqs) */
+    const int* kv_len;       /* [n_seqs] */
+    const int* table;        /* [n_seqs][table_stride] page ids; entries never needed may hold anything */
+    int        table_stride;
+} pickle_cuda_batch_t;
+
+/* Bytes of a pool (0: sizes the pages do not take). */
+PICKLE_CUDA_API size_t pickle_cuda_pages_bytes(int kv_type, int n_pages, int page_size, int n_kv_heads, int head_dim);
+
+/* Write the call's k, v rows (pre-RoPE, row_type) to their pages and give
+ * the rotated q rows: NeoX half-split rotation of the first 2 * half
+ * elements by row `position` of rope_sin / rope_cos [rope_len][half]
+ * (half 0: no rotation, tables unused). The rotated k is rounded to F32
+ * once, then quantised to the nearest code (ties to even). q and q_out may
+ * both be NULL; q_out may be q where the types agree. q [n_tok][n_heads][D],
+ * k, v [n_tok][HK][D]; *_stride: elements between tokens (0: dense). Rows
+ * are 16-byte aligned; half is a multiple of 8. Two rows of one call must
+ * not have the same page position. */
+PICKLE_CUDA_API int  pickle_cuda_pages_append_dev(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch,
+                                                  int n_heads, int row_type, const void* q, size_t q_stride,
+                                                  const void* k, size_t k_stride, const void* v, size_t v_stride,
+                                                  const float* rope_sin, const float* rope_cos, int half, int rope_len,
+                                                  int q_out_type, void* q_out, size_t q_out_stride, void* stream);
+
+/* Read the call's rows back as numbers: k_out, v_out [n_tok][HK][D] of
+ * row_type (rounded once for BF16 rows; 8-bit pages are exact). */
+PICKLE_CUDA_API int  pickle_cuda_pages_read_dev(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch,
+                                                int row_type, void* k_out, size_t k_stride, void* v_out,
+                                                size_t v_stride, void* stream);
+
+/* Attention of the call's (already rotated) q rows over the pages, their own
+ * positions included: out = softmax(q . k / sqrtf(D)) v over the keys at
+ * positions j <= p of a query at position p and, when window > 0, only those
+ * with j > p - window or j < sinks. kv_head = h * HK / H, H / HK from 1 to 8.
+ * q, out [n_tok][n_heads][D] of row_type, accumulation in F32; F32 rows keep
+ * F32 accuracy, BF16 rows round the softmax weights to BF16 where
+ * max_q * H / HK > 8. Pages
+ * that no row of the call can see are never touched (their table entries may
+ * be stale). A row that sees no key gives zeros. Keys on a page outside
+ * the pool are left out and recorded in the error word.
+ * workspace: pickle_cuda_pages_workspace(...) device bytes, 16-byte aligned;
+ * calls that may overlap on the GPU need one each. */
+PICKLE_CUDA_API size_t pickle_cuda_pages_workspace(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch,
+                                                   int n_heads, int row_type, int window, int sinks);
+PICKLE_CUDA_API int  pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch,
+                                                int n_heads, int row_type, const void* q, size_t q_stride, void* out,
+                                                size_t out_stride, int window, int sinks, void* workspace,
+                                                size_t ws_bytes, void* stream);
+
 /* ---- Peer exchange of the sharded decodes (one process per GPU) ----
  * No counterpart in the reference, which runs on one host: this replaces an
  * NCCL all-gather for the small per-step payloads of the KV-head and

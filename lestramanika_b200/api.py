@@ -109,6 +109,12 @@ SIGNATURES = {
     "pickle_cuda_generate_sampled": ([_vp, _i32p, _sz, _i, _i, ctypes.c_float, ctypes.c_float, ctypes.c_uint32,
                                       _i32p, ctypes.POINTER(_i), _fp, ctypes.POINTER(_sz)], _i),
     "pickle_cuda_generate": ([_vp, _i32p, _sz, _i, _i, _i32p, ctypes.POINTER(_i), _fp, ctypes.POINTER(_sz)], _i),
+    "pickle_cuda_pages_bytes": ([_i, _i, _i, _i, _i], _sz),
+    "pickle_cuda_pages_append_dev": ([_vp, _vp, _i, _i, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _i, _i, _i, _vp, _sz,
+                                      _vp], _i),
+    "pickle_cuda_pages_read_dev": ([_vp, _vp, _i, _vp, _sz, _vp, _sz, _vp], _i),
+    "pickle_cuda_pages_workspace": ([_vp, _vp, _i, _i, _i, _i], _sz),
+    "pickle_cuda_pages_attn_dev": ([_vp, _vp, _i, _i, _vp, _sz, _vp, _sz, _i, _i, _vp, _sz, _vp], _i),
     "pickle_cuda_xchg_create": ([_i, _i, _sz, _i, ctypes.POINTER(_vp)], _i),
     "pickle_cuda_xchg_handle": ([_vp, _vp], _i),
     "pickle_cuda_xchg_open": ([_vp, _i, _vp], _i),

@@ -32,7 +32,7 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-UNITS = ("pickle_cuda.cu", "decode_noalloc.cu", "peer_xchg.cu", "matvec.cu", "forward.cu")
+UNITS = ("pickle_cuda.cu", "decode_noalloc.cu", "peer_xchg.cu", "matvec.cu", "forward.cu", "pages.cu")
 
 
 def build_lib(force=False, verbose=False):

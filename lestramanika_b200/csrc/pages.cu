@@ -1,0 +1,390 @@
+// pages.cu - the paged KV cache's entry points (include/pickle_cuda.h), its
+// writer and its reader.
+#include "pages.cuh"
+
+#include <cmath>
+#include <cstring>
+
+#include "pages_attn.cuh"
+
+namespace {
+
+using namespace pages;
+
+// ---- write: rotate, quantise, append --------------------------------------
+
+struct AppendArgs {
+    View w;
+    const void *q, *k, *v;
+    size_t q_stride, k_stride, v_stride;   // elements between tokens
+    void* q_out;
+    size_t q_out_stride;
+    int q_out_bf16;
+    const float *sin_tab, *cos_tab;
+    int H, half, rope_len;
+};
+
+// c * x + s * y rounded once: both products and the sum with their errors
+// (Dekker / Knuth), the errors added last. A code must not depend on how a
+// sum was rounded on the way.
+PCU_DEV float dot2_rn(float c, float x, float s, float y) {
+    const float p = __fmul_rn(c, x), q = __fmul_rn(s, y);
+    const float ep = __fmaf_rn(c, x, -p), eq = __fmaf_rn(s, y, -q);
+    const float d = __fadd_rn(p, q), z = __fsub_rn(d, p);
+    const float e = __fadd_rn(__fsub_rn(p, __fsub_rn(d, z)), __fsub_rn(q, z));
+    const float r = __fadd_rn(d, __fadd_rn(e, __fadd_rn(ep, eq)));
+    return fabsf(d) < INFINITY ? r : d;
+}
+
+template <bool ONCE>
+PCU_DEV float rot(float c, float x, float s, float y) {
+    return ONCE ? dot2_rn(c, x, s, y) : __fmaf_rn(c, x, __fmul_rn(s, y));
+}
+
+template <bool ONCE>
+PCU_DEV void rotate8(Row8& x, const float4 (&c)[2], const float4 (&s)[2], int partner, bool rotated) {
+    Row8 y;
+    y.a = make_float4(__shfl_sync(0xffffffffu, x.a.x, partner), __shfl_sync(0xffffffffu, x.a.y, partner),
+                      __shfl_sync(0xffffffffu, x.a.z, partner), __shfl_sync(0xffffffffu, x.a.w, partner));
+    y.b = make_float4(__shfl_sync(0xffffffffu, x.b.x, partner), __shfl_sync(0xffffffffu, x.b.y, partner),
+                      __shfl_sync(0xffffffffu, x.b.z, partner), __shfl_sync(0xffffffffu, x.b.w, partner));
+    if (!rotated) return;
+    x.a = make_float4(rot<ONCE>(c[0].x, x.a.x, s[0].x, y.a.x), rot<ONCE>(c[0].y, x.a.y, s[0].y, y.a.y),
+                      rot<ONCE>(c[0].z, x.a.z, s[0].z, y.a.z), rot<ONCE>(c[0].w, x.a.w, s[0].w, y.a.w));
+    x.b = make_float4(rot<ONCE>(c[1].x, x.b.x, s[1].x, y.b.x), rot<ONCE>(c[1].y, x.b.y, s[1].y, y.b.y),
+                      rot<ONCE>(c[1].z, x.b.z, s[1].z, y.b.z), rot<ONCE>(c[1].w, x.b.w, s[1].w, y.b.w));
+}
+
+PCU_DEV uint32_t amax_bits(const float4& x) {
+    const uint32_t m = 0x7fffffffu;
+    return max(max(__float_as_uint(x.x) & m, __float_as_uint(x.y) & m), max(__float_as_uint(x.z) & m, __float_as_uint(x.w) & m));
+}
+
+constexpr int APPEND_WARPS = 4;
+
+// One CTA column per token (blockIdx.x); its H + 2 HK rows are spread over
+// the warps of gridDim.y CTAs. D / 8 lanes hold a row, 8 elements each, so a
+// scale's 32 elements are 4 lanes and a rotation partner is half / 8 lanes
+// away. The token's sin / cos stay in registers for all its rows.
+template <int KV, int D, int ROWS>
+__global__ void __launch_bounds__(32 * APPEND_WARPS) pages_append_kernel(const AppendArgs a) {
+    constexpr int LPR = D / 8, RPW = 32 / LPR;
+    const View& w = a.w;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    griddep_wait();
+    griddep_launch_dependents();
+    const int t = blockIdx.x;
+    const int b = seq_of_row(w, t, lane);
+    if (b >= w.n_seqs) return;
+    int row0, n, kv;
+    const bool ok = seq_bounds(w, b, row0, n, kv);
+    const int pos = kv - n + (t - row0);
+    bool live = ok && pos >= 0;
+    if (live && a.half > 0 && pos >= a.rope_len) {
+        record_error(w.err, PCU_DEVERR_ARG);
+        live = false;
+    }
+    const int page = live ? page_of(w, b, pos) : -1;
+    const int sub = lane / LPR, l = lane % LPR, i0 = 8 * l;
+    const int hl = a.half / 8;
+    const bool rotated = l < 2 * hl;
+    const int partner = !rotated ? lane : l < hl ? lane + hl : lane - hl;
+    float4 c[2], s[2];
+    if (live && rotated) {
+        const size_t at = (size_t)pos * a.half + (l < hl ? i0 : i0 - a.half);
+        const float4* sp = reinterpret_cast<const float4*>(a.sin_tab + at);
+        const float4* cp = reinterpret_cast<const float4*>(a.cos_tab + at);
+        const float sg = l < hl ? -1.0f : 1.0f;
+        #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            c[i] = cp[i];
+            s[i] = sp[i];
+            s[i] = make_float4(sg * s[i].x, sg * s[i].y, sg * s[i].z, sg * s[i].w);
+        }
+    }
+    const int HK = w.HK, nq = a.q ? a.H : 0, units = nq + 2 * HK;
+    const int step = gridDim.y * APPEND_WARPS * RPW;
+    for (int u0 = (blockIdx.y * APPEND_WARPS + warp) * RPW; u0 < units; u0 += step) {
+        const int u = u0 + sub;
+        const bool mine = u < units, is_q = u < nq, is_v = u >= nq + HK;
+        const int h = is_q ? u : is_v ? u - nq - HK : u - nq;
+        const void* src = is_q ? a.q : is_v ? a.v : a.k;
+        const size_t stride = is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride;
+        Row8 x;
+        x.a = x.b = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (mine && live) x = load_row8<ROWS>(src, (size_t)t * stride + (size_t)h * D + i0);
+        if (u0 < nq + HK) {          // warp-uniform: some row of this step is a q or k row
+            Row8 y = x;
+            if (u0 + RPW <= nq) {
+                rotate8<false>(y, c, s, partner, live && rotated);
+            } else {
+                rotate8<true>(y, c, s, partner, live && rotated && !is_v);
+            }
+            x = y;
+        }
+        if (mine && is_q) {
+            const size_t at = (size_t)t * a.q_out_stride + (size_t)h * D + i0;
+            if (a.q_out_bf16) store_row8<PICKLE_CUDA_ROW_BF16>(a.q_out, at, x);
+            else store_row8<PICKLE_CUDA_ROW_F32>(a.q_out, at, x);
+        }
+        uint32_t m = 0;
+        if (KV != BF16) {
+            m = max(amax_bits(x.a), amax_bits(x.b));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        }
+        if (mine && !is_q && page >= 0) {
+            const int p = pos % w.page_size, r = p % CELL;
+            unsigned char* cell = cell_ptr<KV, D>(w, page, h, p);
+            if (KV == BF16) {
+                store_row8<PICKLE_CUDA_ROW_BF16>(cell + (is_v ? v_row(KV, D, r) : k_row(KV, D, r)), i0, x);
+            } else {
+                const uint32_t sc = block_scale<KV>(m);
+                *reinterpret_cast<uint2*>(cell + (is_v ? v_row(KV, D, r) : k_row(KV, D, r)) + i0) =
+                    make_uint2(codes4<KV>(x.a, sc), codes4<KV>(x.b, sc));
+                if (l % 4 == 0) cell[(is_v ? v_scale(D, r) : k_scale(D, r)) + i0 / BLOCK] = (unsigned char)sc;
+            }
+        }
+    }
+}
+
+// ---- read back ---------------------------------------------------------------
+
+struct ReadArgs {
+    View w;
+    void *k, *v;
+    size_t k_stride, v_stride;
+};
+
+constexpr int READ_WARPS = 4, READ_AHEAD = 4;
+
+// As the writer: a token per blockIdx.x, D / 8 lanes a row, READ_AHEAD rows
+// in flight per lane.
+template <int KV, int D, int ROWS>
+__global__ void __launch_bounds__(32 * READ_WARPS) pages_read_kernel(const ReadArgs a) {
+    constexpr int LPR = D / 8, RPW = 32 / LPR;
+    const View& w = a.w;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    griddep_wait();
+    griddep_launch_dependents();
+    const int t = blockIdx.x;
+    const int b = seq_of_row(w, t, lane);
+    if (b >= w.n_seqs) return;
+    int row0, n, kv;
+    const bool ok = seq_bounds(w, b, row0, n, kv);
+    const int pos = kv - n + (t - row0);
+    const int page = ok && pos >= 0 ? page_of(w, b, pos) : -1;
+    const int p = page >= 0 ? pos % w.page_size : 0, r = p % CELL;
+    const int sub = lane / LPR, i0 = 8 * (lane % LPR), units = 2 * w.HK;
+    const int step = gridDim.y * READ_WARPS * RPW;
+    for (int u0 = (blockIdx.y * READ_WARPS + warp) * RPW + sub; u0 < units; u0 += READ_AHEAD * step) {
+        Row8 x[READ_AHEAD];
+        #pragma unroll
+        for (int i = 0; i < READ_AHEAD; ++i) {
+            const int u = u0 + i * step;
+            x[i].a = x[i].b = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (u < units && page >= 0) {
+                const bool is_v = u >= w.HK;
+                x[i] = load_cached8<KV, D>(cell_ptr<KV, D>(w, page, is_v ? u - w.HK : u, p), r, i0, is_v);
+            }
+        }
+        #pragma unroll
+        for (int i = 0; i < READ_AHEAD; ++i) {
+            const int u = u0 + i * step;
+            if (u >= units) break;
+            const bool is_v = u >= w.HK;
+            const int h = is_v ? u - w.HK : u;
+            store_row8<ROWS>(is_v ? a.v : a.k, (size_t)t * (is_v ? a.v_stride : a.k_stride) + (size_t)h * D + i0, x[i]);
+        }
+    }
+}
+
+// ---- host ----------------------------------------------------------------------
+
+bool dims_ok(int kv_type, int n_pages, int page_size, int n_kv_heads, int head_dim) {
+    return kv_type >= BF16 && kv_type <= E4M3 && n_pages > 0 && page_size >= CELL && page_size % CELL == 0 &&
+           n_kv_heads > 0 && (head_dim == 64 || head_dim == 128);
+}
+
+int check(const pickle_cuda_pages_t* p, const pickle_cuda_batch_t* b, View* w) {
+    if (!p || !b || !p->pool || (uintptr_t)p->pool % 16 ||
+        !dims_ok(p->kv_type, p->n_pages, p->page_size, p->n_kv_heads, p->head_dim))
+        return PICKLE_ERR_ARG;
+    if (b->n_seqs < 1 || b->n_tok < 0 || b->max_q < 1 || b->max_kv < 0 || b->table_stride < 1 || !b->kv_len || !b->table)
+        return PICKLE_ERR_ARG;
+    if (!b->q_start && (b->max_q != 1 || b->n_tok != b->n_seqs)) return PICKLE_ERR_ARG;
+    if ((long long)b->max_kv > (long long)b->table_stride * p->page_size) return PICKLE_ERR_RANGE;
+    w->pool = (unsigned char*)p->pool;
+    w->n_pages = p->n_pages;
+    w->page_size = p->page_size;
+    w->HK = p->n_kv_heads;
+    w->n_seqs = b->n_seqs;
+    w->n_tok = b->n_tok;
+    w->max_q = b->max_q;
+    w->max_kv = b->max_kv;
+    w->q_start = b->q_start;
+    w->kv_len = b->kv_len;
+    w->table = b->table;
+    w->table_stride = b->table_stride;
+    w->err = p->err;
+    return PICKLE_OK;
+}
+
+// A rows argument: 16-byte aligned, `heads * D` elements per token at least.
+// *stride 0 becomes dense.
+bool rows_ok(const void* ptr, int type, int heads, int D, size_t* stride) {
+    if (!ptr || (uintptr_t)ptr % 16 || (type != PICKLE_CUDA_ROW_F32 && type != PICKLE_CUDA_ROW_BF16)) return false;
+    const size_t dense = (size_t)heads * D;
+    if (*stride == 0) *stride = dense;
+    return *stride >= dense && *stride % (type == PICKLE_CUDA_ROW_F32 ? 4 : 8) == 0;
+}
+
+int sm_count() {
+    static thread_local int dev_of = -1, sms = 0;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev != dev_of) {
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        dev_of = dev;
+    }
+    return sms;
+}
+
+// Launch as a programmatic dependent of the kernel before it on the stream
+// (each kernel waits before its first global access).
+template <class Args>
+int launch(void (*fn)(Args), dim3 grid, int threads, size_t smem, const Args& a, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fn, a) == cudaSuccess ? PICKLE_OK : PICKLE_ERR_DEVICE;
+}
+
+// f(kv type, D, row type) as compile-time constants.
+template <class F>
+int dispatch(int kv, int D, int rows, F f) {
+    auto by_rows = [&](auto k, auto d) {
+        return rows == PICKLE_CUDA_ROW_F32 ? f(k, d, std::integral_constant<int, PICKLE_CUDA_ROW_F32>())
+                                           : f(k, d, std::integral_constant<int, PICKLE_CUDA_ROW_BF16>());
+    };
+    auto by_d = [&](auto k) {
+        return D == 64 ? by_rows(k, std::integral_constant<int, 64>()) : by_rows(k, std::integral_constant<int, 128>());
+    };
+    if (kv == BF16) return by_d(std::integral_constant<int, BF16>());
+    if (kv == I8) return by_d(std::integral_constant<int, I8>());
+    return by_d(std::integral_constant<int, E4M3>());
+}
+
+// CTAs per token: enough to fill the SMs when there are few tokens.
+int ctas_per_token(int n_tok, int units, int units_per_cta) {
+    const int most = (units + units_per_cta - 1) / units_per_cta;
+    const int want = (4 * sm_count() + n_tok - 1) / n_tok;
+    return want < 1 ? 1 : want < most ? want : most;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pickle_cuda_pages_bytes(int kv_type, int n_pages, int page_size, int n_kv_heads, int head_dim) {
+    if (!dims_ok(kv_type, n_pages, page_size, n_kv_heads, head_dim)) return 0;
+    return (size_t)n_pages * n_kv_heads * (page_size / CELL) * cell_bytes(kv_type, head_dim);
+}
+
+int pickle_cuda_pages_append_dev(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch, int n_heads,
+                                 int row_type, const void* q, size_t q_stride, const void* k, size_t k_stride,
+                                 const void* v, size_t v_stride, const float* rope_sin, const float* rope_cos, int half,
+                                 int rope_len, int q_out_type, void* q_out, size_t q_out_stride, void* stream) {
+    AppendArgs a;
+    memset(&a, 0, sizeof(a));
+    int rc = check(pages, batch, &a.w);
+    if (rc != PICKLE_OK) return rc;
+    const int D = pages->head_dim, HK = pages->n_kv_heads;
+    if (!rows_ok(k, row_type, HK, D, &k_stride) || !rows_ok(v, row_type, HK, D, &v_stride)) return PICKLE_ERR_ARG;
+    if ((q == nullptr) != (q_out == nullptr)) return PICKLE_ERR_ARG;
+    if (q && (n_heads < 1 || !rows_ok(q, row_type, n_heads, D, &q_stride) ||
+              !rows_ok(q_out, q_out_type, n_heads, D, &q_out_stride)))
+        return PICKLE_ERR_ARG;
+    if (half < 0 || half % 8 || 2 * half > D || rope_len < 0) return PICKLE_ERR_ARG;
+    if (half > 0 && (!rope_sin || !rope_cos || ((uintptr_t)rope_sin | (uintptr_t)rope_cos) % 16)) return PICKLE_ERR_ARG;
+    if (half > 0 && batch->max_kv > rope_len) return PICKLE_ERR_RANGE;
+    if (batch->n_tok == 0) return PICKLE_OK;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.q_out = q_out;
+    a.q_out_stride = q_out_stride;
+    a.q_out_bf16 = q_out_type == PICKLE_CUDA_ROW_BF16;
+    a.sin_tab = rope_sin;
+    a.cos_tab = rope_cos;
+    a.H = n_heads;
+    a.half = half;
+    a.rope_len = rope_len;
+    const int units = (q ? n_heads : 0) + 2 * HK;
+    const dim3 grid(batch->n_tok, ctas_per_token(batch->n_tok, units, APPEND_WARPS * 256 / D));
+    return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
+        return launch(pages_append_kernel<kv(), d(), rows()>, grid, 32 * APPEND_WARPS, 0, a, (cudaStream_t)stream);
+    });
+}
+
+int pickle_cuda_pages_read_dev(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch, int row_type,
+                               void* k_out, size_t k_stride, void* v_out, size_t v_stride, void* stream) {
+    ReadArgs a;
+    int rc = check(pages, batch, &a.w);
+    if (rc != PICKLE_OK) return rc;
+    const int D = pages->head_dim, HK = pages->n_kv_heads;
+    if (!rows_ok(k_out, row_type, HK, D, &k_stride) || !rows_ok(v_out, row_type, HK, D, &v_stride)) return PICKLE_ERR_ARG;
+    if (batch->n_tok == 0) return PICKLE_OK;
+    a.k = k_out;
+    a.v = v_out;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    const dim3 grid(batch->n_tok, ctas_per_token(batch->n_tok, 2 * HK, READ_WARPS * 256 / D));
+    return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
+        return launch(pages_read_kernel<kv(), d(), rows()>, grid, 32 * READ_WARPS, 0, a, (cudaStream_t)stream);
+    });
+}
+
+size_t pickle_cuda_pages_workspace(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch, int n_heads,
+                                   int row_type, int window, int sinks) {
+    return 0;
+}
+
+int pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch, int n_heads,
+                               int row_type, const void* q, size_t q_stride, void* out, size_t out_stride, int window,
+                               int sinks, void* workspace, size_t ws_bytes, void* stream) {
+    AttnArgs a;
+    memset(&a, 0, sizeof(a));
+    int rc = check(pages, batch, &a.w);
+    if (rc != PICKLE_OK) return rc;
+    const int D = pages->head_dim, HK = pages->n_kv_heads;
+    if (n_heads < 1 || n_heads % HK || n_heads / HK > 8 || window < 0 || sinks < 0) return PICKLE_ERR_ARG;
+    if (!rows_ok(q, row_type, n_heads, D, &q_stride) || !rows_ok(out, row_type, n_heads, D, &out_stride))
+        return PICKLE_ERR_ARG;
+    if (batch->n_tok == 0) return PICKLE_OK;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.H = n_heads;
+    a.G = n_heads / HK;
+    a.window = window;
+    a.sinks = sinks;
+    a.scale_log2 = 1.4426950408889634f / sqrtf((float)D);
+    return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
+        return launch(pages_attn_simple_kernel<kv(), d(), rows()>, dim3(batch->n_tok, n_heads), 32 * SIMPLE_WARPS, 0, a,
+                      (cudaStream_t)stream);
+    });
+}
+
+}  // extern "C"

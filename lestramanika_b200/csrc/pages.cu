@@ -2,10 +2,14 @@
 // writer and its reader.
 #include "pages.cuh"
 
+#include <atomic>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 
 #include "pages_attn.cuh"
+#include "pages_decode.cuh"
+#include "pages_simple.cuh"
 
 namespace {
 
@@ -77,9 +81,9 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS) pages_append_kernel(const A
     const int b = seq_of_row(w, t, lane);
     if (b >= w.n_seqs) return;
     int row0, n, kv;
-    const bool ok = seq_bounds(w, b, row0, n, kv);
+    if (!seq_bounds(w, b, row0, n, kv)) return;
     const int pos = kv - n + (t - row0);
-    bool live = ok && pos >= 0;
+    bool live = pos >= 0;
     if (live && a.half > 0 && pos >= a.rope_len) {
         record_error(w.err, PCU_DEVERR_ARG);
         live = false;
@@ -171,9 +175,9 @@ __global__ void __launch_bounds__(32 * READ_WARPS) pages_read_kernel(const ReadA
     const int b = seq_of_row(w, t, lane);
     if (b >= w.n_seqs) return;
     int row0, n, kv;
-    const bool ok = seq_bounds(w, b, row0, n, kv);
+    if (!seq_bounds(w, b, row0, n, kv)) return;
     const int pos = kv - n + (t - row0);
-    const int page = ok && pos >= 0 ? page_of(w, b, pos) : -1;
+    const int page = pos >= 0 ? page_of(w, b, pos) : -1;
     const int p = page >= 0 ? pos % w.page_size : 0, r = p % CELL;
     const int sub = lane / LPR, i0 = 8 * (lane % LPR), units = 2 * w.HK;
     const int step = gridDim.y * READ_WARPS * RPW;
@@ -282,6 +286,83 @@ int dispatch(int kv, int D, int rows, F f) {
     return by_d(std::integral_constant<int, E4M3>());
 }
 
+// One kernel's shared-memory limit; `done` has a bit per device on which it is set.
+template <class Args>
+int allow_smem(void (*fn)(Args), int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return PICKLE_ERR_DEVICE;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return PICKLE_OK;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return PICKLE_ERR_DEVICE;
+    done.fetch_or(bit, std::memory_order_release);
+    return PICKLE_OK;
+}
+
+struct Plan {
+    bool decode;        // the kernel for few rows
+    int n_splits, chunk;
+};
+
+// How the keys are cut for `groups` independent streams of `steps` steps of
+// `bytes` each, on `slots` CTA slots. A plan's time: waves of CTAs that
+// stream their piece at min(one CTA's rate, HBM / CTAs of the wave) after a
+// fixed ramp, and the join of the pieces.
+int plan_pieces(long long groups, long long steps, double bytes, long long slots, double cta_rate, long long most) {
+    // The same plan is asked for layer after layer, step after step.
+    struct Memo {
+        long long groups, steps, slots, most;
+        double bytes, rate;
+        int pick;
+    };
+    static thread_local Memo memo[16];
+    Memo& k = memo[(unsigned)(groups * 31 + steps) % 16];
+    if (k.pick && k.groups == groups && k.steps == steps && k.slots == slots && k.most == most && k.bytes == bytes &&
+        k.rate == cta_rate)
+        return k.pick;
+    const double hbm = 6.5e12, ramp = 3e-6, join = 3e-6;
+    double best = 1e30;
+    int pick = 1;
+    for (long long s = 1; s <= most && s <= steps; ++s) {
+        const long long chunk = (steps + s - 1) / s;
+        if ((steps + chunk - 1) / chunk != s) continue;
+        const long long n = groups * s, full = n / slots, rem = n % slots;
+        const double piece = (double)chunk * bytes;
+        const double full_rate = cta_rate < hbm / slots ? cta_rate : hbm / slots;
+        double t = full * (piece / full_rate + ramp);
+        if (rem) t += piece / (cta_rate < hbm / rem ? cta_rate : hbm / rem) + ramp;
+        if (s > 1) t += join + (double)s * groups * 8 * 132 * 4 * 2 / hbm;
+        if (t < best) {
+            best = t;
+            pick = (int)s;
+        }
+    }
+    k = Memo{groups, steps, slots, most, bytes, cta_rate, pick};
+    return pick;
+}
+
+Plan plan_attn(const View& w, int kv_type, int D, int G, int window, int sinks) {
+    Plan p;
+    p.decode = true;
+    long long keys = w.max_kv;
+    if (window > 0) {
+        const long long seen = (long long)window + w.max_q + CELL + (sinks < w.max_kv ? sinks : w.max_kv) + CELL;
+        if (seen < keys) keys = seen;
+    }
+    const long long cells = (keys + CELL - 1) / CELL;
+    const int ctas = kv_type == BF16 ? 3 : 2;
+    p.n_splits = plan_pieces((long long)w.n_seqs * w.HK, cells < 1 ? 1 : cells, cell_bytes(kv_type, D),
+                             (long long)sm_count() * ctas, kv_type == BF16 ? 30e9 : 30e9, 64);
+    if (const char* env = getenv("PICKLE_CUDA_PAGES_SPLITS"))
+        if (atoi(env) > 0) p.n_splits = atoi(env);
+    p.chunk = (int)((cells + p.n_splits - 1) / p.n_splits);
+    if (p.chunk < 1) p.chunk = 1;
+    return p;
+}
+
+size_t split_bytes(const View& w, const Plan& p, int H, int D) {
+    return p.n_splits > 1 ? (size_t)p.n_splits * w.n_tok * H * (D + 2) * sizeof(float) : 0;
+}
+
 // CTAs per token: enough to fill the SMs when there are few tokens.
 int ctas_per_token(int n_tok, int units, int units_per_cta) {
     const int most = (units + units_per_cta - 1) / units_per_cta;
@@ -357,7 +438,13 @@ int pickle_cuda_pages_read_dev(const pickle_cuda_pages_t* pages, const pickle_cu
 
 size_t pickle_cuda_pages_workspace(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch, int n_heads,
                                    int row_type, int window, int sinks) {
-    return 0;
+    View w;
+    if (check(pages, batch, &w) != PICKLE_OK || n_heads < 1 || n_heads % w.HK || n_heads / w.HK > 8 || window < 0 ||
+        sinks < 0 || batch->n_tok == 0)
+        return 0;
+    const int G = n_heads / w.HK;
+    if (w.max_q * G > 8) return 0;
+    return split_bytes(w, plan_attn(w, pages->kv_type, pages->head_dim, G, window, sinks), n_heads, pages->head_dim);
 }
 
 int pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch, int n_heads,
@@ -381,9 +468,29 @@ int pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cu
     a.window = window;
     a.sinks = sinks;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)D);
+    const cudaStream_t st = (cudaStream_t)stream;
+    if ((long long)a.w.max_q * a.G > 8)
+        return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
+            return launch(pages_attn_simple_kernel<kv(), d(), rows()>, dim3(batch->n_tok, n_heads), 32 * SIMPLE_WARPS, 0, a, st);
+        });
+    const Plan p = plan_attn(a.w, pages->kv_type, D, a.G, window, sinks);
+    const size_t need = split_bytes(a.w, p, n_heads, D);
+    if (need && (!workspace || (uintptr_t)workspace % 16 || ws_bytes < need)) return PICKLE_ERR_ARG;
+    a.n_splits = p.n_splits;
+    a.chunk = p.chunk;
+    a.ws_o = (float*)workspace;
+    a.ws_ml = a.ws_o + (size_t)p.n_splits * batch->n_tok * n_heads * D;
     return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
-        return launch(pages_attn_simple_kernel<kv(), d(), rows()>, dim3(batch->n_tok, n_heads), 32 * SIMPLE_WARPS, 0, a,
-                      (cudaStream_t)stream);
+        using T = DecodeTile<kv(), d()>;
+        static std::atomic<uint64_t> smem_set{0};
+        int e = allow_smem(pages_decode_kernel<kv(), d(), rows()>, T::SMEM, smem_set);
+        if (e == PICKLE_OK)
+            e = launch(pages_decode_kernel<kv(), d(), rows()>, dim3(a.w.n_seqs * HK, p.n_splits), 32 * T::WARPS, T::SMEM, a, st);
+        if (e == PICKLE_OK && p.n_splits > 1)
+            e = launch(pages_merge_kernel<d(), rows(), CELL>,
+                       dim3((unsigned)(((size_t)batch->n_tok * n_heads + MERGE_WARPS - 1) / MERGE_WARPS)),
+                       32 * MERGE_WARPS, 0, a, st);
+        return e;
     });
 }
 

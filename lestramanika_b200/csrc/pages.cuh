@@ -64,14 +64,19 @@ PCU_DEV int seq_of_row(const View& w, int t, int lane) {
     return b;
 }
 
-// Rows and length of sequence b; false (recorded) where they pass the call's bounds.
+// Rows and length of sequence b. False (recorded) where its rows pass the
+// call's bounds: they are left alone. A length outside the bounds (recorded)
+// counts as 0: no page is touched and the rows lie before position 0.
 PCU_DEV bool seq_bounds(const View& w, int b, int& row0, int& n, int& kv) {
     row0 = w.q_start ? w.q_start[b] : b;
     n = w.q_start ? w.q_start[b + 1] - row0 : 1;
     kv = w.kv_len[b];
-    if (kv <= w.max_kv && kv >= 0 && n <= w.max_q && n >= 0 && row0 >= 0 && row0 + n <= w.n_tok) return true;
-    record_error(w.err, PCU_DEVERR_ARG);
-    return false;
+    const bool rows_ok = n >= 0 && n <= w.max_q && row0 >= 0 && row0 <= w.n_tok - n;
+    if (!rows_ok || kv < 0 || kv > w.max_kv) {
+        record_error(w.err, PCU_DEVERR_ARG);
+        kv = 0;
+    }
+    return rows_ok;
 }
 
 // F32 of a scale byte: 2^(s - 127), NaN for 255.

@@ -59,11 +59,6 @@ PCU_DEV void rotate8(Row8& x, const float4 (&c)[2], const float4 (&s)[2], int pa
                       rot<ONCE>(c[1].z, x.b.z, s[1].z, y.b.z), rot<ONCE>(c[1].w, x.b.w, s[1].w, y.b.w));
 }
 
-PCU_DEV uint32_t amax_bits(const float4& x) {
-    const uint32_t m = 0x7fffffffu;
-    return max(max(__float_as_uint(x.x) & m, __float_as_uint(x.y) & m), max(__float_as_uint(x.z) & m, __float_as_uint(x.w) & m));
-}
-
 constexpr int APPEND_WARPS = 4;
 
 // One CTA column per token (blockIdx.x); its H + 2 HK rows are spread over
@@ -214,6 +209,8 @@ int check(const pickle_cuda_pages_t* p, const pickle_cuda_batch_t* b, View* w) {
     if (!p || !b || !p->pool || (uintptr_t)p->pool % 16 ||
         !dims_ok(p->kv_type, p->n_pages, p->page_size, p->n_kv_heads, p->head_dim))
         return PICKLE_ERR_ARG;
+    // Cells are counted in 32 bits.
+    if ((double)p->n_pages * p->n_kv_heads * (p->page_size / CELL) >= 4294967296.0) return PICKLE_ERR_RANGE;
     if (b->n_seqs < 1 || b->n_tok < 0 || b->max_q < 1 || b->max_kv < 0 || b->table_stride < 1 || !b->kv_len || !b->table)
         return PICKLE_ERR_ARG;
     if (!b->q_start && (b->max_q != 1 || b->n_tok != b->n_seqs)) return PICKLE_ERR_ARG;

@@ -129,6 +129,11 @@ PCU_DEV float4 numbers4(uint32_t c) {
     return x;
 }
 
+PCU_DEV uint32_t amax_bits(const float4& x) {
+    const uint32_t m = 0x7fffffffu;
+    return max(max(__float_as_uint(x.x) & m, __float_as_uint(x.y) & m), max(__float_as_uint(x.z) & m, __float_as_uint(x.w) & m));
+}
+
 // Eight consecutive elements of a row.
 struct Row8 {
     float4 a, b;

@@ -9,18 +9,29 @@
 //     S^T [16 keys][8 rows] = K Q^T,   O^T [16 elements][8 rows] += V^T P^T
 // A warp takes a cell (16 keys) at a time from a ring of its own that it fills
 // with cp.async (no barrier beyond the warp); chunks of a row are swizzled as
-// they are copied, so that fragments are read without bank conflicts. Codes
-// become BF16 numbers in registers: an element is code * 2^e exactly, so
-// nothing is rounded. The order of the d's (of K and Q) and of the d's of an
-// output tile is free, and chosen so that a lane's elements are contiguous.
+// they are copied, so that fragments are read without bank conflicts. The
+// order of the elements of K and Q, and of an output tile, is free, and
+// chosen so that a lane's elements are contiguous.
 //
-// F32 rows keep F32 accuracy: q and the weights p are sums of three BF16
-// numbers (24 bits), each with a product of its own. BF16 rows: q is exact in one,
-// p takes two (16 bits, an error of 2^-17 against the output's own 2^-8).
+// 8-bit codes become F16 numbers in registers: a code is exact in F16, and so
+// is code * 2^(e - E) for a reference exponent E near the largest one seen
+// (elements 2^-24 and more below it lose bits of no weight in the sums). K
+// has one E per warp, which the scores' factor undoes; V has one per 32
+// elements of the output, and moving it rescales O by a power of two. BF16
+// pages are multiplied as they are.
+//
+// F32 rows keep F32 accuracy: q (scaled to a row maximum near 2^15) and the
+// weights p are sums of two F16 numbers (22 bits), each with a product of
+// its own; of three BF16 numbers (24 bits) on BF16 pages. BF16 rows: q is exact
+// in one number; p is one F16 number (its 2^-12 is an eighth of the output's
+// own 2^-8 rounding's root-mean-square) or two BF16 numbers.
 //
 // The running maximum moves only when some score passes it by 2^8 (a warp
-// vote), so most cells need no reduction over the keys at all.
+// vote), so most cells need no reduction over the keys; p is held times 2^7
+// so that small weights stay above F16's subnormals.
 #pragma once
+#include <cuda_fp16.h>
+
 #include "pages_attn.cuh"
 
 namespace pages {
@@ -32,15 +43,13 @@ struct DecodeTile {
     static constexpr int CH = ROWB / 16;              // 16-byte chunks of a row
     static constexpr int KCH = CH / 4;                // chunks of a K row that a lane takes
     static constexpr int CELLB = cell_bytes(KV, D);
-    static constexpr int CPS = 128 / D;               // cells of a ring stage
-    // 8-bit: 16 warps an SM in two CTAs, three stages each (203 KB in all). BF16 cells are twice as large
-    // and cheaper to use: 12 warps in three CTAs, two stages each.
+    // 8-bit: 16 warps an SM in two CTAs with 12 KB of ring each (203 KB in all). BF16 cells are twice as large
+    // and cheaper to use: 12 warps in three CTAs with 16 KB each.
     static constexpr int WARPS = KV == BF16 ? 4 : 8;
     static constexpr int CTAS = KV == BF16 ? 3 : 2;
-    static constexpr int STAGES = KV == BF16 ? 2 : 3;
-    static constexpr int STAGEB = CPS * CELLB;
+    static constexpr int STAGES = (KV == BF16 ? 2 : 3) * 128 / D;
     static constexpr int OPAD = D + 4;                // floats between output columns of a warp's partial
-    static constexpr int RING = WARPS * STAGES * STAGEB;
+    static constexpr int RING = WARPS * STAGES * CELLB;
     static constexpr int JOIN = WARPS * 8 * (OPAD + 2) * 4;
     static constexpr int SMEM = RING > JOIN ? RING : JOIN;
 
@@ -56,10 +65,16 @@ struct DecodeTile {
     }
 };
 
+template <bool BF>
 PCU_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 PCU_DEV uint32_t movmatrix(uint32_t x) {
@@ -73,99 +88,84 @@ PCU_DEV uint32_t bf16x2(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
     return y;
 }
+PCU_DEV uint32_t f16x2(float lo, float hi) {
+    uint32_t y;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+}
+PCU_DEV __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+PCU_DEV uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 
-// Two numbers as N BF16 parts each, largest first: x = part 0 + part 1 + ...
-template <int N>
-PCU_DEV void split_bf16(float lo, float hi, uint32_t (&p)[N]) {
+// Two numbers as N BF16 (or F16) parts each, largest first: x = part 0 + part 1 + ...
+template <bool BF, int N>
+PCU_DEV void split_parts(float lo, float hi, uint32_t (&p)[N]) {
     #pragma unroll
     for (int i = 0; i < N; ++i) {
-        p[i] = bf16x2(lo, hi);
+        p[i] = BF ? bf16x2(lo, hi) : f16x2(lo, hi);
         if (i + 1 < N) {
-            lo -= __uint_as_float(p[i] << 16);
-            hi -= __uint_as_float(p[i] & 0xffff0000u);
+            if (BF) {
+                lo -= __uint_as_float(p[i] << 16);
+                hi -= __uint_as_float(p[i] & 0xffff0000u);
+            } else {
+                const float2 f = __half22float2(as_half2(p[i]));
+                lo -= f.x;
+                hi -= f.y;
+            }
         }
     }
 }
 
-PCU_DEV void fma2(float& a, float& b, float sa, float sb, float ca, float cb) {
-    asm("{\n\t.reg .b64 x, s, c;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\tmov.b64 c, {%4, %5};\n\t"
-        "fma.rn.f32x2 x, x, s, c;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "+f"(a), "+f"(b) : "f"(sa), "f"(sb), "f"(ca), "f"(cb));
-}
+// 2^(e - ref) of scale bytes, as F32; at or below 2^-127 it is 0. e - ref <= 127.
+PCU_DEV float rel_scale(int e, int ref) { return __uint_as_float((uint32_t)max(e - ref + 127, 0) << 23); }
 
-PCU_DEV void mul2(float& a, float& b, float sa, float sb) {
-    asm("{\n\t.reg .b64 x, s;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 s, {%2, %3};\n\t"
-        "mul.rn.f32x2 x, x, s;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "+f"(a), "+f"(b) : "f"(sa), "f"(sb));
-}
-
-// A scale byte as the factor and (I8) the addend that turn 2^23 + 128 + code
-// into code * 2^e, exactly, in one fused multiply-add. 255 (not finite) gives NaN, 0 (a row left out) zero.
-struct Scale {
-    float f, c;
-};
-template <int KV>
-PCU_DEV Scale scale_of(uint32_t byte) {
-    Scale s;
-    s.f = __uint_as_float(byte << 23);
-    s.c = KV == I8 ? -8388736.0f * s.f : 0.f;
-    return s;
-}
-
-// Byte i of offset-binary codes as the float 2^23 + 128 + code.
-template <int I>
-PCU_DEV float magic(uint32_t w) { return __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 + I)); }
-
-PCU_DEV void e4m3x2_f32(uint32_t pair, float& lo, float& hi) {
+PCU_DEV uint32_t e4m3x2_f16x2(uint32_t pair) {
     uint32_t h;
     asm("{\n\t.reg .b16 p, u;\n\tmov.b32 {p, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, p;\n\t}" : "=r"(h) : "r"(pair));
-    asm("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, u;\n\t}"
-        : "=f"(lo), "=f"(hi) : "r"(h));
+    return h;
 }
 
-// Four consecutive codes of a row under one scale -> BF16 pairs (0, 1), (2, 3).
+// Bytes 0 and 2 of x as F16 numbers 1152 + code (the offset-binary code in the low byte of 1024's mantissa).
+PCU_DEV uint32_t i8_magic(uint32_t x) { return (x & 0x00ff00ffu) ^ 0x64806480u; }
+
+// Four consecutive codes of a row, times f (both halves): the pairs of one k-step. I8: elements (0, 2), (1, 3);
+// E4M3: (0, 1), (2, 3). c = -1152 f; the fused product is exact.
 template <int KV>
-PCU_DEV void codes_row(uint32_t w, const Scale& s, uint32_t& p01, uint32_t& p23) {
-    float x0, x1, x2, x3;
+PCU_DEV void codes_row(uint32_t w, uint32_t f, uint32_t c, uint32_t& p0, uint32_t& p1) {
     if (KV == I8) {
-        w ^= 0x80808080u;
-        x0 = magic<0>(w); x1 = magic<1>(w); x2 = magic<2>(w); x3 = magic<3>(w);
-        fma2(x0, x1, s.f, s.f, s.c, s.c);
-        fma2(x2, x3, s.f, s.f, s.c, s.c);
+        p0 = as_u32(__hfma2(as_half2(i8_magic(w)), as_half2(f), as_half2(c)));
+        p1 = as_u32(__hfma2(as_half2(i8_magic(w >> 8)), as_half2(f), as_half2(c)));
     } else {
-        e4m3x2_f32(w, x0, x1);
-        e4m3x2_f32(w >> 16, x2, x3);
-        mul2(x0, x1, s.f, s.f);
-        mul2(x2, x3, s.f, s.f);
+        p0 = as_u32(__hmul2(as_half2(e4m3x2_f16x2(w)), as_half2(f)));
+        p1 = as_u32(__hmul2(as_half2(e4m3x2_f16x2(w >> 16)), as_half2(f)));
     }
-    p01 = bf16x2(x0, x1);
-    p23 = bf16x2(x2, x3);
 }
 
-// Four consecutive codes of two rows -> BF16 pairs (row a, row b) of each element.
+// Four consecutive codes of two rows, times (fa, fb): pairs (row a, row b) of each element.
 template <int KV>
-PCU_DEV void codes_pair(uint32_t wa, uint32_t wb, const Scale& sa, const Scale& sb, uint32_t (&p)[4]) {
-    float a[4], b[4];
+PCU_DEV void codes_pair(uint32_t wa, uint32_t wb, uint32_t f, uint32_t c, uint32_t (&p)[4]) {
     if (KV == I8) {
-        wa ^= 0x80808080u;
-        wb ^= 0x80808080u;
-        a[0] = magic<0>(wa); a[1] = magic<1>(wa); a[2] = magic<2>(wa); a[3] = magic<3>(wa);
-        b[0] = magic<0>(wb); b[1] = magic<1>(wb); b[2] = magic<2>(wb); b[3] = magic<3>(wb);
+        const uint32_t x = __byte_perm(wa, wb, 0x5410), y = __byte_perm(wa, wb, 0x7632);
+        p[0] = i8_magic(x);
+        p[1] = i8_magic(x >> 8);
+        p[2] = i8_magic(y);
+        p[3] = i8_magic(y >> 8);
         #pragma unroll
-        for (int i = 0; i < 4; ++i) fma2(a[i], b[i], sa.f, sb.f, sa.c, sb.c);
+        for (int i = 0; i < 4; ++i) p[i] = as_u32(__hfma2(as_half2(p[i]), as_half2(f), as_half2(c)));
     } else {
-        e4m3x2_f32(wa, a[0], a[1]);
-        e4m3x2_f32(wa >> 16, a[2], a[3]);
-        e4m3x2_f32(wb, b[0], b[1]);
-        e4m3x2_f32(wb >> 16, b[2], b[3]);
+        const uint32_t x = __byte_perm(wa, wb, 0x5140), y = __byte_perm(wa, wb, 0x7362);
+        p[0] = e4m3x2_f16x2(x);
+        p[1] = e4m3x2_f16x2(x >> 16);
+        p[2] = e4m3x2_f16x2(y);
+        p[3] = e4m3x2_f16x2(y >> 16);
         #pragma unroll
-        for (int i = 0; i < 4; ++i) mul2(a[i], b[i], sa.f, sb.f);
+        for (int i = 0; i < 4; ++i) p[i] = as_u32(__hmul2(as_half2(p[i]), as_half2(f)));
     }
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = bf16x2(a[i], b[i]);
 }
 
-PCU_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+PCU_DEV void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+PCU_DEV void cp_async16_or_zero(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 PCU_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -173,31 +173,41 @@ template <int N>
 PCU_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Copy one cell into a ring stage, rows swizzled; rows whose bit of `need`
-// is clear become zeros and their bytes are not read.
+// is clear become zeros and their bytes are not read. The scale bytes come
+// in chunks of several rows, so they are copied if any row is needed (and are
+// ignored for the others).
 template <int KV, int D>
 PCU_DEV void fill_cell(uint32_t dst, const unsigned char* cell, uint32_t need, int lane) {
     using T = DecodeTile<KV, D>;
-    #pragma unroll
-    for (int i = 0; i < 2 * CELL * T::CH / 32; ++i) {
-        const int x = i * 32 + lane, row = x / T::CH, c = x % T::CH, r = row % CELL;
-        cp_async16(dst + row * T::ROWB + T::at(r, c) * 16, cell + x * 16, (need >> r) & 1 ? 16u : 0u);
+    constexpr int N = 2 * CELL * T::CH / 32;
+    const unsigned char* src = cell + lane * 16;
+    if (need == 0xffffu) {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int x = i * 32 + lane, row = x / T::CH, c = x % T::CH;
+            cp_async16(dst + row * T::ROWB + T::at(row % CELL, c) * 16, src + i * 512);
+        }
+    } else {
+        #pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int x = i * 32 + lane, row = x / T::CH, c = x % T::CH, r = row % CELL;
+            cp_async16_or_zero(dst + row * T::ROWB + T::at(r, c) * 16, src + i * 512, (need >> r) & 1 ? 16u : 0u);
+        }
     }
-    if (KV != BF16 && lane < D / CELL) {
-        // 16 scale bytes are 16 / (D / 32) rows: they are copied if any of these rows is needed; a row
-        // left out has codes 0, and the scale of such a row is replaced where it is used.
-        cp_async16(dst + 2 * CELL * T::ROWB + lane * 16, cell + 2 * CELL * D + lane * 16, need ? 16u : 0u);
-    }
+    if (KV != BF16 && lane < D / CELL && need) cp_async16(dst + 2 * CELL * T::ROWB + lane * 16, src + N * 512);
 }
 
 template <int KV, int D, int ROWS>
 __global__ void __launch_bounds__(32 * DecodeTile<KV, D>::WARPS, DecodeTile<KV, D>::CTAS)
 pages_decode_kernel(const AttnArgs a) {
     using T = DecodeTile<KV, D>;
-    constexpr int QP = ROWS == PICKLE_CUDA_ROW_F32 ? 3 : 1, PP = ROWS == PICKLE_CUDA_ROW_F32 ? 3 : 2;
-    constexpr int W = T::WARPS, STAGES = T::STAGES, CPS = T::CPS;
+    constexpr bool BF = KV == BF16, F32 = ROWS == PICKLE_CUDA_ROW_F32;
+    constexpr int QP = !F32 ? 1 : BF ? 3 : 2, PP = BF ? (F32 ? 3 : 2) : (F32 ? 2 : 1);
+    constexpr int W = T::WARPS, STAGES = T::STAGES;
     constexpr int KS = D / 16, MT = D / 16;
+    constexpr int SLACK = 7;              // how far an exponent may pass its reference: 448 * 2^7 is below F16's largest
+    constexpr float P_SHIFT = BF ? 0.f : 7.f, GROW = 8.f;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint32_t s_need[W][STAGES][CPS];
     const View& w = a.w;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     griddep_wait();
@@ -210,115 +220,145 @@ pages_decode_kernel(const AttnArgs a) {
     const int pieces = (span.n + a.chunk - 1) / a.chunk;
     if (split > 0 && split >= pieces) return;
     const int e0 = split * a.chunk, e1 = min(span.n, e0 + a.chunk);
-    const int units = (e1 - e0 + CPS - 1) / CPS;
+    const int mine = (e1 - e0 - warp + W - 1) / W;     // cells e0 + warp, e0 + warp + W, ... of the span
+
+    // What the warp has to know of 32 of its cells, one a lane: where the cell lies in the pool and which of
+    // its keys some row sees. Looking a page up and dividing is done for all of them at once, far ahead.
+    struct Info {
+        uint32_t at;
+        int need;
+    };
+    const uint32_t cpp = w.page_size / CELL;
+    auto look_up = [&](int first) {
+        Info x{0u, 0};
+        const int i = first + lane;
+        if (i < mine) {
+            const uint32_t step = span.step(e0 + warp + i * W);
+            const uint32_t page = step / cpp;
+            const int id = w.table[(size_t)b * w.table_stride + page];
+            if ((unsigned)id < (unsigned)w.n_pages) {
+                const int j0 = step * CELL;
+                uint32_t need = j0 + CELL <= kv ? 0xffffu : (1u << (kv - j0)) - 1u;
+                if (j0 < span.lo_key) {
+                    const uint32_t in = span.lo_key - j0 >= CELL ? 0u : 0xffffu << (span.lo_key - j0);
+                    const uint32_t sk = a.sinks <= j0 ? 0u : a.sinks - j0 >= CELL ? 0xffffu : (1u << (a.sinks - j0)) - 1u;
+                    need &= in | sk;
+                }
+                x.at = ((uint32_t)id * w.HK + hk) * cpp + (step - page * cpp);
+                x.need = (int)need;
+            } else {
+                record_error(w.err, PCU_DEVERR_ARG);
+            }
+        }
+        return x;
+    };
+    const uint32_t ring = smem_u32(smem) + warp * STAGES * T::CELLB;
+    const unsigned char* ring_ptr = smem + warp * STAGES * T::CELLB;
+    auto fill = [&](const Info& x, int i, int slot) {
+        const uint32_t at = __shfl_sync(0xffffffffu, x.at, i & 31);
+        const uint32_t need = (uint32_t)__shfl_sync(0xffffffffu, x.need, i & 31);
+        if (i < mine) fill_cell<KV, D>(ring + slot * T::CELLB, w.pool + (size_t)at * T::CELLB, need, lane);
+    };
+    Info cur = look_up(0);
+    #pragma unroll
+    for (int i = 0; i < STAGES; ++i) {
+        fill(cur, i, i);
+        cp_async_commit();
+    }
+    Info nxt = look_up(32);
 
     // Q^T as B fragments: column g is row g = (token g / G, head g % G).
     uint32_t qf[QP][KS][2];
+    float qs = 1.0f;                       // F16: what the row was multiplied by
     {
-        const bool mine = g < R;
-        const size_t at = (size_t)(row0 + (mine ? g / G : 0)) * a.q_stride + (size_t)(hk * G + (mine ? g % G : 0)) * D;
+        const bool live = g < R;
+        const size_t at = (size_t)(row0 + (live ? g / G : 0)) * a.q_stride + (size_t)(hk * G + (live ? g % G : 0)) * D;
         constexpr int EPC = 16 / T::ES;                // elements of a chunk
+        Row8 x[KS / 2];
         #pragma unroll
-        for (int j = 0; j < T::KCH; ++j)
-            #pragma unroll
-            for (int e = 0; e < EPC; e += 8) {
-                Row8 x;
-                x.a = x.b = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (mine) x = load_row8<ROWS>(a.q, at + T::k_chunk(t, j) * EPC + e);
-                const int ks = (j * EPC + e) / 4;
-                uint32_t p[QP];
-                split_bf16<QP>(x.a.x, x.a.y, p);
-                #pragma unroll
-                for (int i = 0; i < QP; ++i) qf[i][ks][0] = p[i];
-                split_bf16<QP>(x.a.z, x.a.w, p);
-                #pragma unroll
-                for (int i = 0; i < QP; ++i) qf[i][ks][1] = p[i];
-                split_bf16<QP>(x.b.x, x.b.y, p);
-                #pragma unroll
-                for (int i = 0; i < QP; ++i) qf[i][ks + 1][0] = p[i];
-                split_bf16<QP>(x.b.z, x.b.w, p);
-                #pragma unroll
-                for (int i = 0; i < QP; ++i) qf[i][ks + 1][1] = p[i];
-            }
-    }
-
-    const uint32_t ring = smem_u32(smem) + warp * STAGES * T::STAGEB;
-    const unsigned char* ring_ptr = smem + warp * STAGES * T::STAGEB;
-    auto cell_of = [&](int u, int c) { return e0 + u * CPS + c; };      // index into the span
-    auto page_id = [&](int u, int c) {
-        const int e = cell_of(u, c);
-        return u < units && e < e1 ? w.table[(size_t)b * w.table_stride + span.step(e) * CELL / w.page_size] : -1;
-    };
-    auto fill = [&](int u, int slot, const int (&id)[CPS]) {
-        if (u >= units) return;
-        #pragma unroll
-        for (int c = 0; c < CPS; ++c) {
-            const int e = cell_of(u, c);
-            uint32_t need = 0;
-            const unsigned char* src = w.pool;
-            if (e < e1) {
-                const int j0 = span.step(e) * CELL;
-                if ((unsigned)id[c] < (unsigned)w.n_pages) {
-                    // Positions below kv that some row sees.
-                    need = j0 + CELL <= kv ? 0xffffu : (1u << (kv - j0)) - 1u;
-                    if (j0 < span.lo_key) {
-                        const uint32_t in = span.lo_key - j0 >= CELL ? 0u : 0xffffu << (span.lo_key - j0);
-                        const uint32_t sk = a.sinks <= j0 ? 0u : a.sinks - j0 >= CELL ? 0xffffu : (1u << (a.sinks - j0)) - 1u;
-                        need &= in | sk;
-                    }
-                    src = cell_ptr<KV, D>(w, id[c], hk, j0 % w.page_size);
-                } else if (lane == 0) {
-                    record_error(w.err, PCU_DEVERR_ARG);
-                }
-            }
-            if (lane == 0) s_need[warp][slot][c] = need;
-            fill_cell<KV, D>(ring + slot * T::STAGEB + c * T::CELLB, src, need, lane);
+        for (int k = 0; k < KS / 2; ++k) {
+            x[k].a = x[k].b = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (live) x[k] = load_row8<ROWS>(a.q, at + T::k_chunk(t, 8 * k / EPC) * EPC + 8 * k % EPC);
         }
-    };
-
-    // The warp's units: warp, warp + W, ...
-    int ids[STAGES][CPS];
-    #pragma unroll
-    for (int s = 0; s < STAGES; ++s)
+        if (!BF) {
+            uint32_t m = 0;
+            #pragma unroll
+            for (int k = 0; k < KS / 2; ++k) m = max(m, max(amax_bits(x[k].a), amax_bits(x[k].b)));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            // 2^(14 - floor(log2 max)): the largest element comes to lie in [2^14, 2^15).
+            qs = __uint_as_float(min(268u - (m >> 23), 254u) << 23);
+        }
         #pragma unroll
-        for (int c = 0; c < CPS; ++c) ids[s][c] = page_id(warp + s * W, c);
-    int next[CPS];
-    #pragma unroll
-    for (int c = 0; c < CPS; ++c) next[c] = page_id(warp + STAGES * W, c);
-    #pragma unroll
-    for (int s = 0; s < STAGES; ++s) {
-        fill(warp + s * W, s, ids[s]);
-        cp_async_commit();
+        for (int k = 0; k < KS / 2; ++k) {
+            const float v[8] = {x[k].a.x * qs, x[k].a.y * qs, x[k].a.z * qs, x[k].a.w * qs,
+                                x[k].b.x * qs, x[k].b.y * qs, x[k].b.z * qs, x[k].b.w * qs};
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                constexpr int o1 = KV == I8 ? 2 : 1, o2 = KV == I8 ? 1 : 2;      // the pairs codes_row makes
+                uint32_t p[QP];
+                split_parts<BF, QP>(v[4 * h], v[4 * h + o1], p);
+                #pragma unroll
+                for (int i = 0; i < QP; ++i) qf[i][2 * k + h][0] = p[i];
+                split_parts<BF, QP>(v[4 * h + o2], v[4 * h + 3], p);
+                #pragma unroll
+                for (int i = 0; i < QP; ++i) qf[i][2 * k + h][1] = p[i];
+            }
+        }
     }
+    // Scores of the lane's columns (rows 2t, 2t + 1) in log2 units: S * fc. fc0: without K's reference exponent.
+    float fc0[2], fc[2];
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) fc[i] = fc0[i] = a.scale_log2 / __shfl_sync(0xffffffffu, qs, (2 * t + i) * 4);
 
     float o[MT][4];
     #pragma unroll
     for (int i = 0; i < MT; ++i)
         #pragma unroll
         for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, mz[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
-    // Positions of the lane's two columns (rows 2t, 2t + 1 of the call).
+    // m: the maximum that p is relative to (log2 units); mz: what is subtracted; thr: the score (as S) past which m moves.
+    float m[2] = {-INFINITY, -INFINITY}, mz[2] = {0.f, 0.f}, thr[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    int ek = 0, ev = 0;                    // reference exponents (scale bytes) of K (warp) and V (lane group)
     const int pc[2] = {2 * t < R ? pos0 + 2 * t / G : -1, 2 * t + 1 < R ? pos0 + (2 * t + 1) / G : -1};
 
     int slot = 0;
-    for (int u = warp; u < units; u += W) {
+    for (int i = 0; i < mine; ++i) {
+        if (i && (i & 31) == 0) {
+            cur = nxt;
+            nxt = look_up(i + 32);
+        }
+        const uint32_t need = (uint32_t)__shfl_sync(0xffffffffu, cur.need, i & 31);
+        const int j0 = span.step(e0 + warp + i * W) * CELL;
         cp_async_wait<STAGES - 1>();
         __syncwarp();
-        const unsigned char* stage = ring_ptr + slot * T::STAGEB;
-        #pragma unroll
-        for (int c = 0; c < CPS; ++c) {
-            const uint32_t need = s_need[warp][slot][c];
-            if (need == 0) continue;
-            const unsigned char* cell = stage + c * T::CELLB;
-            const int j0 = span.step(cell_of(u, c)) * CELL;
+        if (need) {
+            const unsigned char* cell = ring_ptr + slot * T::CELLB;
             // S^T: A = K rows g, g + 8.
             float sp[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
             {
-                Scale s0, s1;
-                if (KV != BF16) {
+                uint32_t f0 = 0, f1 = 0, c0 = 0, c1 = 0;
+                if (!BF) {
                     const int blk = D == 128 ? t : t >> 1;
-                    s0 = scale_of<KV>(cell[k_scale(D, g) + blk]);
-                    s1 = scale_of<KV>(cell[k_scale(D, g + 8) + blk]);
+                    int x0 = cell[k_scale(D, g) + blk], x1 = cell[k_scale(D, g + 8) + blk];
+                    if (need != 0xffffu) {
+                        x0 = (need >> g) & 1 ? x0 : 0;
+                        x1 = (need >> (g + 8)) & 1 ? x1 : 0;
+                    }
+                    if (__any_sync(0xffffffffu, max(x0, x1) > ek + SLACK)) {
+                        ek = __reduce_max_sync(0xffffffffu, max(x0, x1));
+                        const float f = ek == 255 ? INFINITY : __uint_as_float((uint32_t)ek << 23);
+                        #pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            fc[k] = fmaxf(fc0[k] * f, 1.2e-38f);      // never 0: a masked score is -inf * fc
+                            thr[k] = m[k] == -INFINITY ? m[k] : (m[k] + GROW) / fc[k];
+                        }
+                    }
+                    f0 = f16x2(rel_scale(x0, ek), rel_scale(x0, ek));
+                    f1 = f16x2(rel_scale(x1, ek), rel_scale(x1, ek));
+                    if (KV == I8) {
+                        c0 = as_u32(__hmul2(as_half2(f0), __floats2half2_rn(-1152.f, -1152.f)));
+                        c1 = as_u32(__hmul2(as_half2(f1), __floats2half2_rn(-1152.f, -1152.f)));
+                    }
                 }
                 #pragma unroll
                 for (int j = 0; j < T::KCH; ++j) {
@@ -327,129 +367,151 @@ pages_decode_kernel(const AttnArgs a) {
                     const uint4 y = *reinterpret_cast<const uint4*>(cell + k_row(KV, D, g + 8) + T::at(g + 8, ch) * 16);
                     const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
                     #pragma unroll
-                    for (int e = 0; e < (KV == BF16 ? 2 : 4); ++e) {
-                        const int ks = j * (KV == BF16 ? 2 : 4) + e;
+                    for (int e = 0; e < (BF ? 2 : 4); ++e) {
+                        const int ks = j * (BF ? 2 : 4) + e;
                         uint32_t a0, a1, a2, a3;
-                        if (KV == BF16) {
+                        if (BF) {
                             a0 = xs[2 * e]; a2 = xs[2 * e + 1];
                             a1 = ys[2 * e]; a3 = ys[2 * e + 1];
                         } else {
-                            codes_row<KV>(xs[e], s0, a0, a2);
-                            codes_row<KV>(ys[e], s1, a1, a3);
+                            codes_row<KV>(xs[e], f0, c0, a0, a2);
+                            codes_row<KV>(ys[e], f1, c1, a1, a3);
                         }
                         #pragma unroll
                         for (int p = 0; p < QP; ++p)
-                            mma16816(sp[(QP == 1 ? ks : p) & 1], a0, a1, a2, a3, qf[p][ks][0], qf[p][ks][1]);
+                            mma16816<BF>(sp[(QP == 1 ? ks : p) & 1], a0, a1, a2, a3, qf[p][ks][0], qf[p][ks][1]);
                     }
                 }
             }
             // Scores of keys g (0, 1) and g + 8 (2, 3) for columns 2t, 2t + 1.
             float s[4];
             #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = (sp[0][i] + sp[1][i]) * a.scale_log2;
+            for (int k = 0; k < 4; ++k) s[k] = sp[0][k] + sp[1][k];
             if (need != 0xffffu || j0 + CELL - 1 > pos0 ||
                 (a.window > 0 && j0 <= kv - 1 - a.window && j0 + CELL - 1 >= a.sinks)) {
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = g + 8 * (i >> 1);
-                    if (!((need >> r) & 1) || !sees(pc[i & 1], j0 + r, a.window, a.sinks)) s[i] = -INFINITY;
+                for (int k = 0; k < 4; ++k) {
+                    const int r = g + 8 * (k >> 1);
+                    if (!((need >> r) & 1) || !sees(pc[k & 1], j0 + r, a.window, a.sinks)) s[k] = -INFINITY;
                 }
             }
-            const float top0 = fmaxf(s[0], s[2]), top1 = fmaxf(s[1], s[3]);
-            if (__any_sync(0xffffffffu, top0 > m[0] + 8.0f || top1 > m[1] + 8.0f)) {
-                float x[2] = {fmaxf(top0, m[0]), fmaxf(top1, m[1])};
+            const float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+            if (__any_sync(0xffffffffu, top[0] > thr[0] || top[1] > thr[1])) {
                 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    x[i] = fmaxf(x[i], __shfl_xor_sync(0xffffffffu, x[i], 4));
-                    x[i] = fmaxf(x[i], __shfl_xor_sync(0xffffffffu, x[i], 8));
-                    x[i] = fmaxf(x[i], __shfl_xor_sync(0xffffffffu, x[i], 16));
-                    const float f = x[i] == m[i] ? 1.0f : ex2(m[i] - x[i]);
-                    m[i] = x[i];
-                    mz[i] = x[i] == -INFINITY ? 0.f : x[i];
-                    l[i] *= f;
+                for (int k = 0; k < 2; ++k) {
+                    float x = fmaxf(top[k] == -INFINITY ? top[k] : top[k] * fc[k], m[k]);
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    const float f = x == m[k] ? 1.0f : ex2(m[k] - x);
+                    m[k] = x;
+                    mz[k] = x == -INFINITY ? 0.f : x - P_SHIFT;
+                    thr[k] = x == -INFINITY ? x : (x + GROW) / fc[k];
+                    l[k] *= f;
                     #pragma unroll
-                    for (int k = 0; k < MT; ++k) {
-                        o[k][i] *= f;
-                        o[k][i + 2] *= f;
+                    for (int q = 0; q < MT; ++q) {
+                        o[q][k] *= f;
+                        o[q][k + 2] *= f;
                     }
                 }
             }
             float p[4];
             #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = ex2(s[i] - mz[i & 1]);
+            for (int k = 0; k < 4; ++k) p[k] = ex2(fmaf(s[k], fc[k & 1], -mz[k & 1]));
             l[0] += p[0] + p[2];
             l[1] += p[1] + p[3];
             // P^T as B fragments: rows (columns of S^T) by keys.
             uint32_t pf[2][PP];
-            split_bf16<PP>(p[0], p[1], pf[0]);
-            split_bf16<PP>(p[2], p[3], pf[1]);
+            split_parts<BF, PP>(p[0], p[1], pf[0]);
+            split_parts<BF, PP>(p[2], p[3], pf[1]);
             #pragma unroll
-            for (int i = 0; i < PP; ++i) {
-                pf[0][i] = movmatrix(pf[0][i]);
-                pf[1][i] = movmatrix(pf[1][i]);
+            for (int k = 0; k < PP; ++k) {
+                pf[0][k] = movmatrix(pf[0][k]);
+                pf[1][k] = movmatrix(pf[1][k]);
             }
             // O^T: A = V^T, keys 2t, 2t + 1, 2t + 8, 2t + 9 of the lane's elements.
             const int rk[4] = {2 * t, 2 * t + 1, 2 * t + 8, 2 * t + 9};
-            Scale sv[4];
-            if (KV != BF16) {
-                const int blk = D == 128 ? g >> 1 : g >> 2;
-                #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    sv[i] = scale_of<KV>((need >> rk[i]) & 1 ? cell[v_scale(D, rk[i]) + blk] : 0);
-            }
-            if (KV == BF16) {
+            if (BF) {
                 #pragma unroll
                 for (int half = 0; half < D / 64; ++half) {
                     uint4 x[4];
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        x[i] = *reinterpret_cast<const uint4*>(cell + v_row(KV, D, rk[i]) + T::at(rk[i], g + 8 * half) * 16);
+                    for (int k = 0; k < 4; ++k)
+                        x[k] = *reinterpret_cast<const uint4*>(cell + v_row(KV, D, rk[k]) + T::at(rk[k], g + 8 * half) * 16);
                     #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t x0 = (&x[0].x)[e], x1 = (&x[1].x)[e], x2 = (&x[2].x)[e], x3 = (&x[3].x)[e];
                         const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
                         const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
                         #pragma unroll
-                        for (int i = 0; i < PP; ++i) mma16816(o[4 * half + e], a0, a1, a2, a3, pf[0][i], pf[1][i]);
+                        for (int k = 0; k < PP; ++k) mma16816<BF>(o[4 * half + e], a0, a1, a2, a3, pf[0][k], pf[1][k]);
                     }
                 }
             } else {
+                const int blk = D == 128 ? g >> 1 : g >> 2;
+                int x4[4];
+                #pragma unroll
+                for (int k = 0; k < 4; ++k) x4[k] = cell[v_scale(D, rk[k]) + blk];
+                if (need != 0xffffu) {
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) x4[k] = (need >> rk[k]) & 1 ? x4[k] : 0;
+                }
+                int top_e = max(max(x4[0], x4[1]), max(x4[2], x4[3]));
+                if (__any_sync(0xffffffffu, top_e > ev + SLACK)) {
+                    // The four lanes of a group share their output rows.
+                    top_e = max(top_e, __shfl_xor_sync(0xffffffffu, top_e, 1));
+                    top_e = max(top_e, __shfl_xor_sync(0xffffffffu, top_e, 2));
+                    top_e = max(top_e, ev);
+                    const float f = rel_scale(ev, top_e);
+                    ev = top_e;
+                    #pragma unroll
+                    for (int q = 0; q < MT; ++q)
+                        #pragma unroll
+                        for (int k = 0; k < 4; ++k) o[q][k] *= f;
+                }
+                const uint32_t f0 = f16x2(rel_scale(x4[0], ev), rel_scale(x4[1], ev));
+                const uint32_t f1 = f16x2(rel_scale(x4[2], ev), rel_scale(x4[3], ev));
+                uint32_t c0 = 0, c1 = 0;
+                if (KV == I8) {
+                    c0 = as_u32(__hmul2(as_half2(f0), __floats2half2_rn(-1152.f, -1152.f)));
+                    c1 = as_u32(__hmul2(as_half2(f1), __floats2half2_rn(-1152.f, -1152.f)));
+                }
                 constexpr int VW = D / 32;                 // words of codes per key
                 uint32_t x[4][VW];
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int k = 0; k < 4; ++k) {
                     if (D == 128) {
-                        const uint4 y = *reinterpret_cast<const uint4*>(cell + v_row(KV, D, rk[i]) + T::at(rk[i], g) * 16);
-                        x[i][0] = y.x; x[i][1] = y.y; x[i][VW - 2] = y.z; x[i][VW - 1] = y.w;
+                        const uint4 y = *reinterpret_cast<const uint4*>(cell + v_row(KV, D, rk[k]) + T::at(rk[k], g) * 16);
+                        x[k][0] = y.x; x[k][1] = y.y; x[k][VW - 2] = y.z; x[k][VW - 1] = y.w;
                     } else {
-                        const uint2 y = *reinterpret_cast<const uint2*>(cell + v_row(KV, D, rk[i]) +
-                                                                        T::at(rk[i], g >> 1) * 16 + (g & 1) * 8);
-                        x[i][0] = y.x; x[i][1] = y.y;
+                        const uint2 y = *reinterpret_cast<const uint2*>(cell + v_row(KV, D, rk[k]) +
+                                                                        T::at(rk[k], g >> 1) * 16 + (g & 1) * 8);
+                        x[k][0] = y.x; x[k][1] = y.y;
                     }
                 }
                 #pragma unroll
                 for (int e = 0; e < VW; ++e) {
                     uint32_t lo[4], hi[4];
-                    codes_pair<KV>(x[0][e], x[1][e], sv[0], sv[1], lo);
-                    codes_pair<KV>(x[2][e], x[3][e], sv[2], sv[3], hi);
+                    codes_pair<KV>(x[0][e], x[1][e], f0, c0, lo);
+                    codes_pair<KV>(x[2][e], x[3][e], f1, c1, hi);
                     #pragma unroll
-                    for (int i = 0; i < PP; ++i) {
-                        mma16816(o[2 * e], lo[0], lo[1], hi[0], hi[1], pf[0][i], pf[1][i]);
-                        mma16816(o[2 * e + 1], lo[2], lo[3], hi[2], hi[3], pf[0][i], pf[1][i]);
+                    for (int k = 0; k < PP; ++k) {
+                        mma16816<BF>(o[2 * e], lo[0], lo[1], hi[0], hi[1], pf[0][k], pf[1][k]);
+                        mma16816<BF>(o[2 * e + 1], lo[2], lo[3], hi[2], hi[3], pf[0][k], pf[1][k]);
                     }
                 }
             }
         }
         __syncwarp();
-        fill(u + STAGES * W, slot, next);
+        const int ahead = i + STAGES;
+        fill((ahead ^ i) & ~31 ? nxt : cur, ahead, slot);
         cp_async_commit();
-        #pragma unroll
-        for (int c = 0; c < CPS; ++c) next[c] = page_id(u + (STAGES + 1) * W, c);
         slot = slot + 1 == STAGES ? 0 : slot + 1;
     }
     cp_async_wait<0>();
 
     // Join the warps: partial (m, l, O) of each through shared memory.
+    const float vf = BF ? 1.0f : ev == 255 ? INFINITY : __uint_as_float((uint32_t)ev << 23);
     #pragma unroll
     for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
@@ -465,7 +527,7 @@ pages_decode_kernel(const AttnArgs a) {
         #pragma unroll
         for (int k = 0; k < MT; ++k) {
             // elements 2k, 2k + 1 of the lane's run are adjacent
-            *reinterpret_cast<float2*>(dst + T::v_elem(g, 2 * k)) = make_float2(o[k][i], o[k][i + 2]);
+            *reinterpret_cast<float2*>(dst + T::v_elem(g, 2 * k)) = make_float2(o[k][i] * vf, o[k][i + 2] * vf);
         }
         if (g == 0) {
             s_ml[(warp * 8 + 2 * t + i) * 2] = m[i];

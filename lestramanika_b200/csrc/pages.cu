@@ -8,8 +8,8 @@
 #include <cstring>
 
 #include "pages_attn.cuh"
+#include "pages_chunk.cuh"
 #include "pages_decode.cuh"
-#include "pages_simple.cuh"
 
 namespace {
 
@@ -296,63 +296,102 @@ int allow_smem(void (*fn)(Args), int bytes, std::atomic<uint64_t>& done) {
 }
 
 struct Plan {
-    bool decode;        // the kernel for few rows
+    bool few;           // the kernel for few rows
+    int blocks;         // else: blocks of rows a sequence may have
     int n_splits, chunk;
 };
 
-// How the keys are cut for `groups` independent streams of `steps` steps of
-// `bytes` each, on `slots` CTA slots. A plan's time: waves of CTAs that
-// stream their piece at min(one CTA's rate, HBM / CTAs of the wave) after a
-// fixed ramp, and the join of the pieces.
-int plan_pieces(long long groups, long long steps, double bytes, long long slots, double cta_rate, long long most) {
+// How many pieces the keys of `groups` independent streams of `steps` steps
+// are cut into, on `slots` CTA slots: waves of CTAs of the same length. A
+// step takes step_s alone in its slot, or what HBM needs for the wave's
+// bytes; a wave adds a ramp, several pieces add the join and its traffic.
+struct Costs {
+    double step_s, step_bytes, ramp_s, join_s, join_bytes;
+};
+int plan_pieces(long long groups, long long steps, long long slots, const Costs& c) {
     // The same plan is asked for layer after layer, step after step.
     struct Memo {
-        long long groups, steps, slots, most;
-        double bytes, rate;
+        long long groups, steps, slots;
+        double a, b;
         int pick;
     };
     static thread_local Memo memo[16];
-    Memo& k = memo[(unsigned)(groups * 31 + steps) % 16];
-    if (k.pick && k.groups == groups && k.steps == steps && k.slots == slots && k.most == most && k.bytes == bytes &&
-        k.rate == cta_rate)
+    Memo& k = memo[(unsigned long long)(groups * 31 + steps) % 16];
+    if (k.pick && k.groups == groups && k.steps == steps && k.slots == slots && k.a == c.step_s && k.b == c.join_bytes)
         return k.pick;
-    const double hbm = 6.5e12, ramp = 3e-6, join = 3e-6;
+    const double hbm = 6.5e12;
+    const int most = steps < 64 ? (int)steps : 64;
     double best = 1e30;
     int pick = 1;
-    for (long long s = 1; s <= most && s <= steps; ++s) {
+    for (int s = 1; s <= most; ++s) {
         const long long chunk = (steps + s - 1) / s;
         if ((steps + chunk - 1) / chunk != s) continue;
         const long long n = groups * s, full = n / slots, rem = n % slots;
-        const double piece = (double)chunk * bytes;
-        const double full_rate = cta_rate < hbm / slots ? cta_rate : hbm / slots;
-        double t = full * (piece / full_rate + ramp);
-        if (rem) t += piece / (cta_rate < hbm / rem ? cta_rate : hbm / rem) + ramp;
-        if (s > 1) t += join + (double)s * groups * 8 * 132 * 4 * 2 / hbm;
+        auto wave = [&](long long ctas) {
+            const double alone = c.step_s * chunk, bytes = c.step_bytes * chunk * ctas / hbm;
+            return (alone > bytes ? alone : bytes) + c.ramp_s;
+        };
+        double t = full * wave(slots) + (rem ? wave(rem) : 0.0);
+        if (s > 1) t += c.join_s + s * c.join_bytes / hbm;
         if (t < best) {
             best = t;
-            pick = (int)s;
+            pick = s;
         }
     }
-    k = Memo{groups, steps, slots, most, bytes, cta_rate, pick};
+    k = Memo{groups, steps, slots, c.step_s, c.join_bytes, pick};
     return pick;
 }
 
-Plan plan_attn(const View& w, int kv_type, int D, int G, int window, int sinks) {
+// Tile sizes of the kernel for many rows, by types.
+struct ChunkDims {
+    int bn, rows;
+};
+ChunkDims chunk_dims(int kv_type, int D, int row_type) {
+    ChunkDims d = {0, 0};
+    dispatch(kv_type, D, row_type, [&](auto kv, auto dd, auto rows) {
+        using T = ChunkTile<kv(), dd(), rows()>;
+        d = {T::BN, T::ROWS_CTA};
+        return 0;
+    });
+    return d;
+}
+
+Plan plan_attn(const View& w, int kv_type, int D, int row_type, int H, int window, int sinks) {
     Plan p;
-    p.decode = true;
+    const int G = H / w.HK;
+    p.few = (long long)w.max_q * G <= 8;
+    const ChunkDims cd = p.few ? ChunkDims{CELL, 8} : chunk_dims(kv_type, D, row_type);
+    p.blocks = (int)(((long long)w.max_q * G + cd.rows - 1) / cd.rows);
+    // The most keys that a block's rows can see.
     long long keys = w.max_kv;
     if (window > 0) {
-        const long long seen = (long long)window + w.max_q + CELL + (sinks < w.max_kv ? sinks : w.max_kv) + CELL;
+        const long long tokens = p.few ? w.max_q : cd.rows / G + 2;
+        const long long seen = (long long)window + tokens + (sinks < w.max_kv ? sinks : w.max_kv) + 2 * cd.bn;
         if (seen < keys) keys = seen;
     }
-    const long long cells = (keys + CELL - 1) / CELL;
-    const int ctas = kv_type == BF16 ? 3 : 2;
-    p.n_splits = plan_pieces((long long)w.n_seqs * w.HK, cells < 1 ? 1 : cells, cell_bytes(kv_type, D),
-                             (long long)sm_count() * ctas, kv_type == BF16 ? 30e9 : 30e9, 64);
+    const long long steps = keys < 1 ? 1 : (keys + cd.bn - 1) / cd.bn;
+    const long long groups = (long long)w.n_seqs * w.HK * p.blocks;
+    const double bytes = (double)cell_bytes(kv_type, D) * (cd.bn / CELL);
+    Costs c;
+    c.step_bytes = bytes;
+    c.join_bytes = 2.0 * w.n_tok * H * D * 4;
+    int slots = sm_count();
+    if (p.few) {
+        // One CTA streams at most 33 GB/s.
+        c.step_s = bytes / 33e9;
+        c.ramp_s = 3e-6;
+        c.join_s = 3e-6;
+        slots *= kv_type == BF16 ? 3 : 2;
+    } else {
+        c.step_s = (row_type == PICKLE_CUDA_ROW_F32 ? 2.0e-6 : 1.2e-6) * cd.bn / 128;
+        c.ramp_s = 5e-6;
+        c.join_s = 4e-6;
+    }
+    p.n_splits = plan_pieces(groups, steps, slots < 1 ? 1 : slots, c);
+    // Knob for sweeps of the piece count.
     if (const char* env = getenv("PICKLE_CUDA_PAGES_SPLITS"))
-        if (atoi(env) > 0) p.n_splits = atoi(env);
-    p.chunk = (int)((cells + p.n_splits - 1) / p.n_splits);
-    if (p.chunk < 1) p.chunk = 1;
+        if (atoi(env) > 0) p.n_splits = atoi(env) < steps ? atoi(env) : (int)steps;
+    p.chunk = (int)((steps + p.n_splits - 1) / p.n_splits);
     return p;
 }
 
@@ -437,11 +476,10 @@ size_t pickle_cuda_pages_workspace(const pickle_cuda_pages_t* pages, const pickl
                                    int row_type, int window, int sinks) {
     View w;
     if (check(pages, batch, &w) != PICKLE_OK || n_heads < 1 || n_heads % w.HK || n_heads / w.HK > 8 || window < 0 ||
-        sinks < 0 || batch->n_tok == 0)
+        sinks < 0 || batch->n_tok == 0 || (row_type != PICKLE_CUDA_ROW_F32 && row_type != PICKLE_CUDA_ROW_BF16))
         return 0;
-    const int G = n_heads / w.HK;
-    if (w.max_q * G > 8) return 0;
-    return split_bytes(w, plan_attn(w, pages->kv_type, pages->head_dim, G, window, sinks), n_heads, pages->head_dim);
+    return split_bytes(w, plan_attn(w, pages->kv_type, pages->head_dim, row_type, n_heads, window, sinks), n_heads,
+                       pages->head_dim);
 }
 
 int pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch, int n_heads,
@@ -455,6 +493,7 @@ int pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cu
     if (n_heads < 1 || n_heads % HK || n_heads / HK > 8 || window < 0 || sinks < 0) return PICKLE_ERR_ARG;
     if (!rows_ok(q, row_type, n_heads, D, &q_stride) || !rows_ok(out, row_type, n_heads, D, &out_stride))
         return PICKLE_ERR_ARG;
+    if ((long long)batch->max_q * (n_heads / HK) > (1 << 22)) return PICKLE_ERR_RANGE;
     if (batch->n_tok == 0) return PICKLE_OK;
     a.q = q;
     a.out = out;
@@ -466,27 +505,32 @@ int pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cu
     a.sinks = sinks;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)D);
     const cudaStream_t st = (cudaStream_t)stream;
-    if ((long long)a.w.max_q * a.G > 8)
-        return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
-            return launch(pages_attn_simple_kernel<kv(), d(), rows()>, dim3(batch->n_tok, n_heads), 32 * SIMPLE_WARPS, 0, a, st);
-        });
-    const Plan p = plan_attn(a.w, pages->kv_type, D, a.G, window, sinks);
+    const Plan p = plan_attn(a.w, pages->kv_type, D, row_type, n_heads, window, sinks);
     const size_t need = split_bytes(a.w, p, n_heads, D);
     if (need && (!workspace || (uintptr_t)workspace % 16 || ws_bytes < need)) return PICKLE_ERR_ARG;
     a.n_splits = p.n_splits;
     a.chunk = p.chunk;
     a.ws_o = (float*)workspace;
     a.ws_ml = a.ws_o + (size_t)p.n_splits * batch->n_tok * n_heads * D;
+    const dim3 merge_grid((unsigned)(((size_t)batch->n_tok * n_heads + MERGE_WARPS - 1) / MERGE_WARPS));
     return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
-        using T = DecodeTile<kv(), d()>;
-        static std::atomic<uint64_t> smem_set{0};
-        int e = allow_smem(pages_decode_kernel<kv(), d(), rows()>, T::SMEM, smem_set);
+        static std::atomic<uint64_t> few_set{0}, many_set{0};
+        if (p.few) {
+            using T = DecodeTile<kv(), d()>;
+            const auto fn = pages_decode_kernel<kv(), d(), rows()>;
+            int e = allow_smem(fn, T::SMEM, few_set);
+            if (e == PICKLE_OK) e = launch(fn, dim3(a.w.n_seqs * HK, p.n_splits), 32 * T::WARPS, T::SMEM, a, st);
+            if (e == PICKLE_OK && p.n_splits > 1)
+                e = launch(pages_merge_kernel<d(), rows(), CELL, 0>, merge_grid, 32 * MERGE_WARPS, 0, a, st);
+            return e;
+        }
+        using T = ChunkTile<kv(), d(), rows()>;
+        const auto fn = pages_chunk_kernel<kv(), d(), rows()>;
+        int e = allow_smem(fn, T::SMEM, many_set);
         if (e == PICKLE_OK)
-            e = launch(pages_decode_kernel<kv(), d(), rows()>, dim3(a.w.n_seqs * HK, p.n_splits), 32 * T::WARPS, T::SMEM, a, st);
+            e = launch(fn, dim3(a.w.n_seqs * HK, p.blocks, p.n_splits), CHUNK_THREADS, T::SMEM, a, st);
         if (e == PICKLE_OK && p.n_splits > 1)
-            e = launch(pages_merge_kernel<d(), rows(), CELL>,
-                       dim3((unsigned)(((size_t)batch->n_tok * n_heads + MERGE_WARPS - 1) / MERGE_WARPS)),
-                       32 * MERGE_WARPS, 0, a, st);
+            e = launch(pages_merge_kernel<d(), rows(), T::BN, T::ROWS_CTA>, merge_grid, 32 * MERGE_WARPS, 0, a, st);
         return e;
     });
 }

@@ -55,4 +55,27 @@ PCU_DEV bool sees(int p, int j, int window, int sinks) {
     return j <= p && (window <= 0 || j > p - window || j < sinks);
 }
 
+// The rows and keys of one block of ROWS_CTA rows (a row: a token and a query
+// head of its KV head's group), for the kernel that takes them in blocks.
+struct ChunkWork {
+    int row0, R, pos0;        // the sequence's first row in the buffers, its rows of a KV head, first position
+    int r0;                   // first row of the block
+    Span span;
+    int last;                 // position of the block's last row
+    int pieces;
+};
+
+template <int BN, int ROWS_CTA>
+PCU_DEV ChunkWork chunk_work(const AttnArgs& a, int row0, int n, int kv, int qb) {
+    ChunkWork c;
+    c.row0 = row0;
+    c.R = n * a.G;
+    c.pos0 = kv - n;
+    c.r0 = qb * ROWS_CTA;
+    c.last = c.pos0 + min(c.R - 1, c.r0 + ROWS_CTA - 1) / a.G;
+    c.span = span_of<BN>(max(0, c.pos0 + c.r0 / a.G), c.last, a.window, a.sinks);
+    c.pieces = (c.span.n + a.chunk - 1) / a.chunk;
+    return c;
+}
+
 }  // namespace pages

@@ -574,7 +574,8 @@ pages_decode_kernel(const AttnArgs a) {
 // pieces that never ran are never read.
 constexpr int MERGE_WARPS = 4;
 
-template <int D, int ROWS, int STEP>
+// ROWS_CTA: rows of the split kernel's blocks (0: it takes a sequence's rows together).
+template <int D, int ROWS, int STEP, int ROWS_CTA>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) pages_merge_kernel(const AttnArgs a) {
     constexpr int E = D / 32;
     const View& w = a.w;
@@ -588,8 +589,12 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) pages_merge_kernel(const Att
     if (b >= w.n_seqs) return;
     int row0, n, kv;
     if (!seq_bounds(w, b, row0, n, kv)) return;
-    const Span span = span_of<STEP>(max(0, kv - n), kv - 1, a.window, a.sinks);
-    const int pieces = (span.n + a.chunk - 1) / a.chunk;
+    int pieces;
+    if constexpr (ROWS_CTA > 0) {
+        pieces = chunk_work<STEP, ROWS_CTA>(a, row0, n, kv, ((tok - row0) * a.G + head % a.G) / ROWS_CTA).pieces;
+    } else {
+        pieces = (span_of<STEP>(max(0, kv - n), kv - 1, a.window, a.sinks).n + a.chunk - 1) / a.chunk;
+    }
     if (pieces <= 1) return;
     // lane i holds piece i's statistics (pieces beyond 32: the loop below takes 32 at a time)
     float M = -INFINITY;

@@ -501,6 +501,7 @@ int pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cu
     a.out_stride = out_stride;
     a.H = n_heads;
     a.G = n_heads / HK;
+    a.inv_g = a.G == 1 ? 0u : (uint32_t)(((1ull << 32) + a.G - 1) / a.G);
     a.window = window;
     a.sinks = sinks;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)D);

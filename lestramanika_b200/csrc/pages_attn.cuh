@@ -14,6 +14,7 @@ struct AttnArgs {
     void* out;
     size_t q_stride, out_stride;
     int H, G;
+    uint32_t inv_g;       // ceil(2^32 / G), 0 for G = 1
     int window, sinks;
     float scale_log2;     // log2(e) / sqrtf(D)
     int n_splits;         // most pieces a sequence's keys are cut into
@@ -27,6 +28,9 @@ PCU_DEV float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// row / G for rows below 2^29: the multiply's error, row * (G - 1) / 2^32, stays below 1 / G.
+PCU_DEV int div_group(int row, const AttnArgs& a) { return a.inv_g ? (int)__umulhi((uint32_t)row, a.inv_g) : row; }
 
 // The keys that the rows at positions first..last can see, in steps of STEP
 // keys: steps [0, sunk) and [lo, end) of the sequence, `n` in all. Without a

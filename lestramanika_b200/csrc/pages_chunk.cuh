@@ -61,6 +61,9 @@ constexpr int CHUNK_THREADS = 512;
 constexpr int CHUNK_STAGE_WARP = 8, CHUNK_MMA_WARP = 12;
 // Registers a thread after the split: 8 softmax, 4 staging, 4 other warps; 32 * (8 * 176 + 4 * 112 + 4 * 48) = 65536,
 // what 512 threads of 128 were launched with.
+// The lowest n bits, n of any size or sign.
+PCU_DEV uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+PCU_DEV void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 PCU_DEV void sts128(uint32_t to, const uint4& v) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -104,6 +107,41 @@ PCU_DEV void tmem_ld64(uint32_t taddr, float* v) {
     for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// 128 consecutive 32-bit columns of this thread's TMEM lane, two loads in flight together.
+PCU_DEV void tmem_ld2x64(uint32_t taddr, float* v) {
+    uint32_t r[128];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%128];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%129];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+          "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]),
+          "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]),
+          "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]),
+          "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]),
+          "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
+          "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        : "r"(taddr), "r"(taddr + 64)
+        : "memory");
+    #pragma unroll
+    for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 PCU_DEV void tmem_st16(uint32_t taddr, const uint32_t* v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -129,16 +167,19 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) pages_chunk_kernel(const Att
     constexpr int NP = T::NP, BN = T::BN, STAGES = T::STAGES, NB = D / 32;
     constexpr float P_SHIFT = BF ? 0.f : 7.f, GROW = 8.f;
     constexpr int SLACK = 7;
-    enum { Q_FULL = 0, S_FULL = 2, P_LO = 4, P_HI = 6, O_DONE = 8, DRAIN = 10, KV_FULL = 11, KV_EMPTY = KV_FULL + STAGES,
-           N_BARS = KV_EMPTY + STAGES };
+    enum { Q_FULL = 0, S_FULL = 2, P_LO = 4, P_HI = 6, O_DONE = 8, DRAIN = 10, K_FULL = 11, K_EMPTY = K_FULL + STAGES,
+           V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES, N_BARS = V_EMPTY + STAGES };
     static_assert(N_BARS * 8 <= 256, "barriers");
+    // What staging tells the softmax of a tile outlives the tile's K: K's stage is free once its S is made, while the
+    // softmax of that S still runs. A slot comes up again only after the S of STAGES tiles later.
+    constexpr int INFO = 2 * STAGES;
     extern __shared__ unsigned char smem_raw[];
     // What staging tells the softmax of a stage: K's factors (one per staging warp), V's O factors (if any moved), V's
     // references, the keys that are really there.
-    __shared__ __align__(16) float s_kf[STAGES][4], s_vf[STAGES][4], s_ve[STAGES][4];
-    __shared__ uint32_t s_there[STAGES][4];
-    __shared__ int s_flag[STAGES];                // 1: V's references moved; 2: keys on a bad page
-    __shared__ uint32_t s_vmax[2][4];
+    __shared__ __align__(16) float s_kf[INFO][4], s_vf[INFO][4], s_ve[INFO][4];
+    __shared__ uint32_t s_there[INFO][4];
+    __shared__ int s_flag[INFO];                // 1: V's references moved; 2: keys on a bad page
+    __shared__ __align__(16) uint32_t s_vmax[2][4];
     __shared__ int s_stop[2];                     // a staging warp gave up: the four leave at the same tile
     __shared__ int s_abort;
     __shared__ uint32_t s_tmem;
@@ -169,15 +210,17 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) pages_chunk_kernel(const Att
     if (tid == 0) {
         for (int x = 0; x < 2; ++x) {
             mbar_init(&bars[Q_FULL + x], 4);
-            mbar_init(&bars[S_FULL + x], 1);
+            mbar_init(&bars[S_FULL + x], 2);      // the products, and the thread that saw the tile's words
             mbar_init(&bars[P_LO + x], 4);
             mbar_init(&bars[P_HI + x], 4);
             mbar_init(&bars[O_DONE + x], 1);
         }
         mbar_init(&bars[DRAIN], 1);
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&bars[KV_FULL + s], 4);
-            mbar_init(&bars[KV_EMPTY + s], 1);
+            mbar_init(&bars[K_FULL + s], 4);
+            mbar_init(&bars[V_FULL + s], 4);
+            mbar_init(&bars[K_EMPTY + s], 1);
+            mbar_init(&bars[V_EMPTY + s], 1);
         }
         mbar_fence_init();
         s_abort = s_stop[0] = s_stop[1] = 0;
@@ -205,6 +248,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) pages_chunk_kernel(const Att
                                  smem_desc(base_u32 + (x * NP + p) * T::Q_TILE + (ks / 4) * T::Q_HALF + (ks % 4) * 32, 16, 1024),
                                  smem_desc(kv_addr(j) + (ks / 4) * T::KV_HALF + (ks % 4) * 32, 16, 1024), id_s, p > 0 || ks > 0);
                 mma_commit(&bars[S_FULL + x]);
+                mbar_arrive(&bars[S_FULL + x]);
+                // The last tile of rows that reads this K lets it go.
+                if (x == 1 || j >= n_b) mma_commit(&bars[K_EMPTY + j % STAGES]);
             };
             auto issue_o = [&](int x, int j, int ks0) {
                 #pragma unroll
@@ -219,18 +265,18 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) pages_chunk_kernel(const Att
                     }
             };
             bool ok = true;
-            int kv_ready = -1;
-            auto wait_kv = [&](int j) {
-                if (ok && j > kv_ready) {
-                    ok = mbar_wait(&bars[KV_FULL + j % STAGES], (j / STAGES) & 1);
-                    kv_ready = j;
+            int k_ready = -1, v_ready = -1;
+            auto wait_tile = [&](int bar, int& ready, int j) {
+                if (ok && j > ready) {
+                    ok = mbar_wait(&bars[bar + j % STAGES], (j / STAGES) & 1);
+                    ready = j;
                 }
                 tc_fence_after();
             };
             for (int x = 0; x < 2 && ok; ++x)
                 if (x ? n_b : n_a) {
                     ok = mbar_wait(&bars[Q_FULL + x], 0);
-                    wait_kv(0);
+                    wait_tile(K_FULL, k_ready, 0);
                     if (ok) issue_s(x, 0);
                 }
             for (int j = 0; ok && j < n_all; ++j) {
@@ -238,21 +284,20 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) pages_chunk_kernel(const Att
                     const int n_x = x ? n_b : n_a;
                     if (j >= n_x) continue;
                     ok = mbar_wait(&bars[P_LO + x], j & 1);
+                    wait_tile(V_FULL, v_ready, j);
                     if (!ok) break;
-                    tc_fence_after();
                     issue_o(x, j, 0);
                     ok = mbar_wait(&bars[P_HI + x], j & 1);
                     if (!ok) break;
                     tc_fence_after();
                     issue_o(x, j, BN / 32);
-                    if (j + 1 == n_x) {
-                        mma_commit(&bars[O_DONE + x]);
-                    } else {
-                        wait_kv(j + 1);
+                    if (j + 1 == n_x) mma_commit(&bars[O_DONE + x]);
+                    if (x == 1 || j >= n_b) mma_commit(&bars[V_EMPTY + j % STAGES]);
+                    if (j + 1 < n_x) {
+                        wait_tile(K_FULL, k_ready, j + 1);
                         if (ok) issue_s(x, j + 1);
                     }
                 }
-                if (ok) mma_commit(&bars[KV_EMPTY + j % STAGES]);
             }
             if (!ok) fail(PCU_DEVERR_MMA_WAIT);
             mma_commit(&bars[DRAIN]);
@@ -264,92 +309,130 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) pages_chunk_kernel(const Att
         constexpr int KPW = BN / 4;                                 // keys of a tile that this warp brings
         const int sw = warp - CHUNK_STAGE_WARP;
         const uint32_t cpp = w.page_size / CELL;
-        // Lane i looks after key i of the warp's: its cell in the pool, or NONE where no row sees it.
+        // Lane i looks after key i of the warp's: its cell in the pool, or NONE where no row sees it. A page id is
+        // asked for a tile before it is turned into a cell, so that nothing waits for the table.
         constexpr uint32_t NONE = 0xffffffffu;
+        struct Ask {
+            int id, cell_in_page;            // cell_in_page < 0: no row sees the key
+        };
         struct Look {
             uint32_t at;
             bool bad;
         };
-        auto look_up = [&](int j) {
-            Look x{NONE, false};
+        // The pages of the warp's keys: KPW / CELL cells, so only one division a tile and lane.
+        auto ask = [&](int j) {
+            Ask x{0, -1};
             if (j < n_all && lane < KPW) {
                 const int key = cw.span.step(t0 + j) * BN + sw * KPW + lane;
                 if (key <= cw.last && (key >= cw.span.lo_key || key < a.sinks)) {
                     const uint32_t cell = (uint32_t)key / CELL, page = cell / cpp;
-                    const int id = w.table[(size_t)b * w.table_stride + page];
-                    x.bad = (unsigned)id >= (unsigned)w.n_pages;
-                    if (!x.bad) x.at = ((uint32_t)id * w.HK + hk) * cpp + (cell - page * cpp);
+                    x.id = w.table[(size_t)b * w.table_stride + page];
+                    x.cell_in_page = (int)(cell - page * cpp);
                 }
             }
             return x;
+        };
+        auto look = [&](const Ask& q) {
+            Look x{NONE, false};
+            if (q.cell_in_page >= 0) {
+                x.bad = (unsigned)q.id >= (unsigned)w.n_pages;
+                if (!x.bad) x.at = ((uint32_t)q.id * w.HK + hk) * cpp + q.cell_in_page;
+            }
+            return x;
+        };
+        // Ask for a tile's rows in L2 (a lane its key's): the copies that come two tiles later then find them there
+        // instead of waiting for DRAM with only a tile in flight.
+        auto prefetch = [&](const Look& x) {
+            if (x.at == NONE) return;
+            const unsigned char* cell = w.pool + (size_t)x.at * cell_bytes(KV, D);
+            const int r = lane % CELL;
+            #pragma unroll
+            for (int i = 0; i < D * elem_bytes(KV); i += 128) {
+                prefetch_l2(cell + k_row(KV, D, r) + i);
+                prefetch_l2(cell + v_row(KV, D, r) + i);
+            }
+            if (!BF && r == 0) prefetch_l2(cell + k_scale(D, 0));
         };
         auto row_ptr = [&](uint32_t at, int row, bool v) {
             return w.pool + (size_t)at * cell_bytes(KV, D) + (v ? v_row(KV, D, row % CELL) : k_row(KV, D, row % CELL));
         };
         bool ok = true;
         // Tell the softmax which keys are missing although some row sees them.
-        auto publish = [&](int s, const Look& x, int moved) {
+        auto publish = [&](int i, const Look& x, int moved) {
             const uint32_t there = __ballot_sync(0xffffffffu, x.at != NONE);
             const uint32_t bad = __ballot_sync(0xffffffffu, x.bad);
             if (lane == 0) {
-                s_there[s][sw] = there;
+                s_there[i][sw] = there;
                 if (bad) {
-                    atomicOr(&s_flag[s], 2);
+                    atomicOr(&s_flag[i], 2);
                     record_error(w.err, PCU_DEVERR_ARG);
                 }
-                if (moved) atomicOr(&s_flag[s], 1);
+                if (moved) atomicOr(&s_flag[i], 1);
             }
         };
-        auto full = [&](int j) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars[KV_FULL + j % STAGES]);
+        auto wait_empty = [&](int bar, int j) {
+            if (ok && j >= STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&bars[bar + j % STAGES], ((j / STAGES) - 1) & 1));
         };
-        // Wait until tile j's stage is empty, clear its flag, and meet the other staging warps; false: all four stop.
+        // Wait until tile j's K may be written, clear its words, and meet the other staging warps; false: all four stop.
         auto begin = [&](int j) {
-            if (j >= STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&bars[KV_EMPTY + j % STAGES], ((j / STAGES) - 1) & 1));
+            wait_empty(K_EMPTY, j);
             if (lane == 0) {
                 if (!ok || aborted()) *(volatile int*)&s_stop[j & 1] = 1;
-                if (sw == 0) *(volatile int*)&s_flag[j % STAGES] = 0;
+                if (sw == 0) *(volatile int*)&s_flag[j % INFO] = 0;
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             return *(volatile int*)&s_stop[j & 1] == 0;
         };
+        auto full = [&](int bar, int j) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[bar + j % STAGES]);
+        };
         if constexpr (BF) {
             constexpr int CPR = D / 8, RPI = 32 / CPR, NI = KPW / RPI;
-            Look nxt = look_up(0);
-            // A tile is announced LAG tiles after its copies went out. Tile j's stage empties only after tile
-            // j - STAGES + 1 has been announced (its S is issued between the products that free the stage).
-            constexpr int LAG = STAGES - 2;
-            for (int j = 0; j < n_all + LAG; ++j) {
+            Ask far = ask(2);
+            Look x = look(ask(0)), nxt = look(ask(1));
+            prefetch(nxt);
+            // Step 2j copies tile j's K, step 2j + 1 its V; a step is announced LAG steps after its copies went out.
+            // V(j) waits for the products of tile j - STAGES, which wait for K(j - STAGES + 1), so LAG is 2 at most.
+            constexpr int LAG = 2;
+            for (int step = 0; step < 2 * n_all + LAG; ++step) {
+                const int j = step >> 1, v = step & 1;
                 if (j < n_all) {
-                    const Look x = nxt;
-                    nxt = look_up(j + 1);
-                    if (!begin(j)) break;
-                    const int s = j % STAGES;
-                    publish(s, x, 0);
-                    const uint32_t dst = base_u32 + T::SMEM_KV + s * T::STAGE;
+                    if (v == 0) {
+                        if (!begin(j)) break;
+                        publish(j % INFO, x, 0);
+                    } else {
+                        wait_empty(V_EMPTY, j);
+                    }
+                    const uint32_t dst = base_u32 + T::SMEM_KV + (j % STAGES) * T::STAGE + v * T::KV_TILE;
                     #pragma unroll
-                    for (int v = 0; v < 2; ++v)
-                        #pragma unroll
-                        for (int i = 0; i < NI; ++i) {
-                            const int row = i * RPI + lane / CPR, c = lane % CPR, r = sw * KPW + row;
-                            const uint32_t at = __shfl_sync(0xffffffffu, x.at, row);
-                            const uint32_t to = dst + v * T::KV_TILE + (c >> 3) * T::KV_HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                            cp_async16_or_zero(to, at == NONE ? w.pool : row_ptr(at, row, v) + c * 16, at == NONE ? 0u : 16u);
-                        }
+                    for (int i = 0; i < NI; ++i) {
+                        const int row = i * RPI + lane / CPR, c = lane % CPR, r = sw * KPW + row;
+                        const uint32_t at = __shfl_sync(0xffffffffu, x.at, row);
+                        const uint32_t to = dst + (c >> 3) * T::KV_HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                        cp_async16_or_zero(to, at == NONE ? w.pool : row_ptr(at, row, v) + c * 16, at == NONE ? 0u : 16u);
+                    }
+                    if (v) {
+                        x = nxt;
+                        nxt = look(far);
+                        prefetch(nxt);
+                        far = ask(j + 3);
+                    }
                 }
                 cp_async_commit();
-                if (j >= LAG) {
+                if (step >= LAG) {
                     cp_async_wait<LAG>();
-                    full(j - LAG);
+                    full((step - LAG) & 1 ? V_FULL : K_FULL, (step - LAG) >> 1);
                 }
             }
             cp_async_wait<0>();
         } else {
             constexpr int CPR = D / 16, RPI = 32 / CPR, NI = KPW / RPI;
             uint32_t ev = 0;                       // V's reference exponents, a byte per 32 elements
-            Look x0 = look_up(0), x1 = look_up(1);
+            Ask far = ask(2);
+            Look x0 = look(ask(0)), x1 = look(ask(1));
+            prefetch(x1);
             uint32_t ks0 = 0, vs0 = 0, ks1 = 0, vs1 = 0;
             auto scales = [&](const Look& x, uint32_t& ks, uint32_t& vs) {
                 ks = vs = 0;
@@ -398,47 +481,44 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) pages_chunk_kernel(const Att
             scales(x0, ks0, vs0);
             load(x0, false, kq);
             for (int j = 0; j < n_all; ++j) {
-                const int s = j % STAGES;
+                const int i = j % INFO;
                 load(x0, true, vq);
                 scales(x1, ks1, vs1);
-                const Look x2 = look_up(j + 2);
+                const Look x2 = look(far);
+                prefetch(x2);
+                far = ask(j + 3);
                 // K: one reference for the warp's keys. V: the tile's maxima, through shared memory.
-                uint32_t km = ks0;
+                uint32_t km = ks0 & 255u;
                 #pragma unroll
-                for (int k = 1; k < NB; ++k) km = max(km & 255u, (ks0 >> (8 * k)) & 255u);
-                km = __reduce_max_sync(0xffffffffu, km & 255u);
+                for (int k = 1; k < NB; ++k) km = max(km, (ks0 >> (8 * k)) & 255u);
+                km = __reduce_max_sync(0xffffffffu, km);
                 uint32_t vm = 0;
                 #pragma unroll
                 for (int k = 0; k < NB; ++k)
                     vm |= __reduce_max_sync(0xffffffffu, (vs0 >> (8 * k)) & 255u) << (8 * k);
                 if (lane == 0) s_vmax[j & 1][sw] = vm;
                 if (!begin(j)) break;
-                int moved = 0;
-                float vf[4] = {1.f, 1.f, 1.f, 1.f};
-                #pragma unroll
-                for (int k = 0; k < NB; ++k) {
-                    const uint32_t old = (ev >> (8 * k)) & 255u;
-                    uint32_t top = 0;
-                    #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = max(top, (s_vmax[j & 1][i] >> (8 * k)) & 255u);
-                    if (top > old + SLACK) {
-                        moved = 1;
-                        vf[k] = rel_scale((int)old, (int)top);
-                        ev = (ev & ~(255u << (8 * k))) | (top << (8 * k));
-                    }
-                }
-                publish(s, x0, sw == 0 && moved);
-                if (lane == 0) s_kf[s][sw] = km == 255u ? INFINITY : __uint_as_float(km << 23);
+                // Every thread keeps all of V's references; lane k of warp 0 tells the softmax about block k.
+                const uint4 vm4 = *reinterpret_cast<const uint4*>(s_vmax[j & 1]);
+                const uint32_t top4 = __vmaxu4(__vmaxu4(vm4.x, vm4.y), __vmaxu4(vm4.z, vm4.w));
+                const uint32_t old4 = ev;
+                // Saturated bytes: top > old + SLACK.
+                const uint32_t past = __vcmpgtu4(top4, __vaddus4(old4, 0x01010101u * SLACK));
+                ev = (old4 & ~past) | (top4 & past);
+                publish(i, x0, sw == 0 && past != 0);
+                if (lane == 0) s_kf[i][sw] = km == 255u ? INFINITY : __uint_as_float(km << 23);
                 if (sw == 0 && lane < NB) {
-                    const uint32_t e = (ev >> (8 * lane)) & 255u;
-                    s_ve[s][lane] = e == 255u ? INFINITY : __uint_as_float(e << 23);
-                    s_vf[s][lane] = lane == 0 ? vf[0] : lane == 1 ? vf[1] : lane == 2 ? vf[2] : vf[3];
+                    const uint32_t e = (ev >> (8 * lane)) & 255u, o = (old4 >> (8 * lane)) & 255u;
+                    s_ve[i][lane] = e == 255u ? INFINITY : __uint_as_float(e << 23);
+                    s_vf[i][lane] = rel_scale((int)o, (int)e);
                 }
-                const uint32_t dst = base_u32 + T::SMEM_KV + s * T::STAGE;
+                const uint32_t dst = base_u32 + T::SMEM_KV + (j % STAGES) * T::STAGE;
                 store(dst, kq, ks0, km * 0x01010101u);
+                full(K_FULL, j);
                 load(x1, false, kq);
+                wait_empty(V_EMPTY, j);
                 store(dst + T::KV_TILE, vq, vs0, ev);
-                full(j);
+                full(V_FULL, j);
                 x0 = x1;
                 x1 = x2;
                 ks0 = ks1;
@@ -460,38 +540,50 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) pages_chunk_kernel(const Att
         bool ok = true;
         float rf = a.scale_log2;
         if (n_x > 0) {
-            // This thread's q row into shared memory, in the operand order.
-            const size_t at = live ? (size_t)(cw.row0 + tok) * a.q_stride + (size_t)head * D : 0;
-            float qs = 1.f;
-            if (!BF) {
-                uint32_t m = 0;
-                if (live) {
-                    #pragma unroll 4
-                    for (int i = 0; i < D; i += 8) {
-                        const Row8 v = load_row8<ROWS>(a.q, at + i);
-                        m = max(m, max(amax_bits(v.a), amax_bits(v.b)));
+            // The warp's 32 q rows into shared memory, in the operand order: D / 8 lanes a row, eight steps in flight.
+            constexpr int LPR = D / 8, RPS = 32 / LPR, STEPS = 32 / RPS;
+            const int i0 = 8 * (lane % LPR), wr0 = cw.r0 + x * 128 + (warp & 3) * 32;
+            float my_qs = 1.f;
+            #pragma unroll 1
+            for (int s0 = 0; s0 < STEPS; s0 += 8) {
+                Row8 v[8];
+                #pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int q = wr0 + (s0 + k) * RPS + lane / LPR;
+                    v[k].a = v[k].b = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (q < cw.R)
+                    {
+                        const int t = div_group(q, a);
+                        v[k] = load_row8<ROWS>(a.q, (size_t)(cw.row0 + t) * a.q_stride + (size_t)(hk * a.G + q - t * a.G) * D + i0);
                     }
                 }
-                qs = __uint_as_float(min(268u - (m >> 23), 254u) << 23);
-                rf = a.scale_log2 / qs;
-            }
-            #pragma unroll 2
-            for (int i = 0; i < D; i += 8) {
-                Row8 v;
-                v.a = v.b = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (live) v = load_row8<ROWS>(a.q, at + i);
-                const float e[8] = {v.a.x * qs, v.a.y * qs, v.a.z * qs, v.a.w * qs, v.b.x * qs, v.b.y * qs, v.b.z * qs, v.b.w * qs};
-                constexpr int o1 = KV == I8 ? 2 : 1, o2 = KV == I8 ? 1 : 2;
-                uint32_t q0[NP], q1[NP], q2[NP], q3[NP];
-                split_parts<BF, NP>(e[0], e[o1], q0);
-                split_parts<BF, NP>(e[o2], e[3], q1);
-                split_parts<BF, NP>(e[4], e[4 + o1], q2);
-                split_parts<BF, NP>(e[4 + o2], e[7], q3);
-                const int c = operand_pos<KV, D>(i) >> 3;            // 16-byte chunk of the row
-                const uint32_t to = base_u32 + x * NP * T::Q_TILE + (c >> 3) * T::Q_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
                 #pragma unroll
-                for (int k = 0; k < NP; ++k) sts128(to + k * T::Q_TILE, make_uint4(q0[k], q1[k], q2[k], q3[k]));
+                for (int k = 0; k < 8; ++k) {
+                    const int rr = (s0 + k) * RPS + lane / LPR;              // row of the warp
+                    float qs = 1.f;
+                    if (!BF) {
+                        uint32_t m = max(amax_bits(v[k].a), amax_bits(v[k].b));
+                        #pragma unroll
+                        for (int y = 1; y < LPR; y <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, y));
+                        qs = __uint_as_float(min(268u - (m >> 23), 254u) << 23);
+                        const float theirs = __shfl_sync(0xffffffffu, qs, (lane % RPS) * LPR);
+                        if (lane / RPS == s0 + k) my_qs = theirs;
+                    }
+                    const float e[8] = {v[k].a.x * qs, v[k].a.y * qs, v[k].a.z * qs, v[k].a.w * qs,
+                                        v[k].b.x * qs, v[k].b.y * qs, v[k].b.z * qs, v[k].b.w * qs};
+                    constexpr int o1 = KV == I8 ? 2 : 1, o2 = KV == I8 ? 1 : 2;
+                    uint32_t q0[NP], q1[NP], q2[NP], q3[NP];
+                    split_parts<BF, NP>(e[0], e[o1], q0);
+                    split_parts<BF, NP>(e[o2], e[3], q1);
+                    split_parts<BF, NP>(e[4], e[4 + o1], q2);
+                    split_parts<BF, NP>(e[4 + o2], e[7], q3);
+                    const int c = operand_pos<KV, D>(i0) >> 3, r_t = (warp & 3) * 32 + rr;      // 16-byte chunk, row of the tile
+                    const uint32_t to = base_u32 + x * NP * T::Q_TILE + (c >> 3) * T::Q_HALF + r_t * 128 + (((c & 7) ^ (r_t & 7)) << 4);
+                    #pragma unroll
+                    for (int y = 0; y < NP; ++y) sts128(to + y * T::Q_TILE, make_uint4(q0[y], q1[y], q2[y], q3[y]));
+                }
             }
+            rf = a.scale_log2 / my_qs;
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars[Q_FULL + x]);
@@ -502,26 +594,27 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) pages_chunk_kernel(const Att
         float m_run = -INFINITY, l_run = 0.f;
         float4 ve = make_float4(1.f, 1.f, 1.f, 1.f);
         for (int j = 0; j < n_x; ++j) {
-            const int s = j % STAGES;
-            ok = __all_sync(0xffffffffu, mbar_wait(&bars[S_FULL + x], j & 1) && mbar_wait(&bars[KV_FULL + s], (j / STAGES) & 1));
+            const int s = j % INFO;
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars[S_FULL + x], j & 1));
             if (!ok) break;
             tc_fence_after();
             float sc[BN];
-            #pragma unroll
-            for (int c = 0; c < BN / 64; ++c) tmem_ld64(s_tm + c * 64, sc + c * 64);
+            if constexpr (BN == 128) tmem_ld2x64(s_tm, sc);
+            else tmem_ld64(s_tm, sc);
             const int j0 = cw.span.step(t0 + j) * BN;
             const int flag = *(volatile int*)&s_flag[s];
             if (j0 + BN - 1 > p_first || (a.window > 0 && j0 <= p_last - a.window && j0 + BN - 1 >= a.sinks) || (flag & 2)) {
-                // Columns past the row's position, and those before its window that are no sinks.
+                // The row's visible columns as bits: at or before its position, inside its window or among the
+                // sinks, and really there. Two instructions a column then.
                 const int hi = max(p, -1) - j0, sk = a.sinks - j0;
                 const int lo = (a.window > 0 ? max(max(p, -1) - a.window, -1) : -1) - j0;
                 #pragma unroll
-                for (int c = 0; c < BN; ++c)
-                    if (c > hi || (c <= lo && c >= sk)) sc[c] = -INFINITY;
-                if (flag & 2) {
+                for (int k = 0; k < BN / 32; ++k) {
+                    uint32_t see = bits_below(hi + 1 - 32 * k) & (~bits_below(lo + 1 - 32 * k) | bits_below(sk - 32 * k));
+                    if (flag & 2) see &= BN == 128 ? s_there[s][k] : s_there[s][2 * k] | s_there[s][2 * k + 1] << 16;
                     #pragma unroll
-                    for (int c = 0; c < BN; ++c)
-                        if (!((s_there[s][c / (BN / 4)] >> (c % (BN / 4))) & 1)) sc[c] = -INFINITY;
+                    for (int c = 0; c < 32; ++c)
+                        if (!(see & (1u << c))) sc[32 * k + c] = -INFINITY;
                 }
             }
             // Factors of the four key groups; never 0, a masked score is -inf times it.
@@ -613,13 +706,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1) pages_chunk_kernel(const Att
                     const int rr = 4 * i + (lane >> 3), q = wr0 + rr;
                     const uint4 v = lds128(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
                     if (q < cw.R) {
-                        const size_t tk = cw.row0 + q / a.G, hd = hk * a.G + q % a.G;
+                        const int t = div_group(q, a), tk = cw.row0 + t, hd = hk * a.G + q - t * a.G;
                         if constexpr (decltype(f32)::value) {
-                            float* to = whole ? reinterpret_cast<float*>(a.out) + tk * a.out_stride + hd * D
-                                              : a.ws_o + (split * rows + tk * a.H + hd) * D;
+                            float* to = whole ? reinterpret_cast<float*>(a.out) + (size_t)tk * a.out_stride + hd * D
+                                              : a.ws_o + (split * rows + (size_t)tk * a.H + hd) * D;
                             *reinterpret_cast<uint4*>(to + d0 + 4 * (lane & 7)) = v;
                         } else {
-                            __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(a.out) + tk * a.out_stride + hd * D;
+                            __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)tk * a.out_stride + hd * D;
                             *reinterpret_cast<uint4*>(to + d0 + 8 * (lane & 7)) = v;
                         }
                     }

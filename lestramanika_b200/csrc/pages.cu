@@ -2,6 +2,9 @@
 // writer and its reader.
 #include "pages.cuh"
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <atomic>
 #include <cmath>
 #include <cstdlib>
@@ -209,8 +212,9 @@ int check(const pickle_cuda_pages_t* p, const pickle_cuda_batch_t* b, View* w) {
     if (!p || !b || !p->pool || (uintptr_t)p->pool % 16 ||
         !dims_ok(p->kv_type, p->n_pages, p->page_size, p->n_kv_heads, p->head_dim))
         return PICKLE_ERR_ARG;
-    // Cells are counted in 32 bits.
-    if ((double)p->n_pages * p->n_kv_heads * (p->page_size / CELL) >= 4294967296.0) return PICKLE_ERR_RANGE;
+    // Cells are counted in 32 bits, rows of a BF16 pool in a tensor copy's signed 32.
+    if ((double)p->n_pages * p->n_kv_heads * (p->page_size / CELL) >= (p->kv_type == BF16 ? 67108864.0 : 4294967296.0))
+        return PICKLE_ERR_RANGE;
     if (b->n_seqs < 1 || b->n_tok < 0 || b->max_q < 1 || b->max_kv < 0 || b->table_stride < 1 || !b->kv_len || !b->table)
         return PICKLE_ERR_ARG;
     if (!b->q_start && (b->max_q != 1 || b->n_tok != b->n_seqs)) return PICKLE_ERR_ARG;
@@ -251,10 +255,18 @@ int sm_count() {
     return sms;
 }
 
+// T itself, from which no template argument is deduced.
+template <class T>
+struct same {
+    using type = T;
+};
+template <class T>
+using same_t = typename same<T>::type;
+
 // Launch as a programmatic dependent of the kernel before it on the stream
 // (each kernel waits before its first global access).
-template <class Args>
-int launch(void (*fn)(Args), dim3 grid, int threads, size_t smem, const Args& a, cudaStream_t st) {
+template <class... Args>
+int launch(void (*fn)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t st, const same_t<Args>&... a) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -265,7 +277,7 @@ int launch(void (*fn)(Args), dim3 grid, int threads, size_t smem, const Args& a,
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fn, a) == cudaSuccess ? PICKLE_OK : PICKLE_ERR_DEVICE;
+    return cudaLaunchKernelEx(&cfg, fn, a...) == cudaSuccess ? PICKLE_OK : PICKLE_ERR_DEVICE;
 }
 
 // f(kv type, D, row type) as compile-time constants.
@@ -284,8 +296,8 @@ int dispatch(int kv, int D, int rows, F f) {
 }
 
 // One kernel's shared-memory limit; `done` has a bit per device on which it is set.
-template <class Args>
-int allow_smem(void (*fn)(Args), int bytes, std::atomic<uint64_t>& done) {
+template <class... Args>
+int allow_smem(void (*fn)(Args...), int bytes, std::atomic<uint64_t>& done) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return PICKLE_ERR_DEVICE;
     const uint64_t bit = dev < 64 ? 1ull << dev : 0;
@@ -399,6 +411,31 @@ size_t split_bytes(const View& w, const Plan& p, int H, int D) {
     return p.n_splits > 1 ? (size_t)p.n_splits * w.n_tok * H * (D + 2) * sizeof(float) : 0;
 }
 
+// The pool's rows as a tensor of [rows][D] BF16 numbers, boxes of 64 columns
+// and a cell's 16 rows in the 128-byte swizzle. Zero for 8-bit pages, which
+// are not read through it.
+int rows_map(CUtensorMap* map, const pickle_cuda_pages_t* p) {
+    memset(map, 0, sizeof(*map));
+    if (p->kv_type != BF16) return PICKLE_OK;
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> encode{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 fn = encode.load(std::memory_order_acquire);
+    if (!fn) {
+        void* sym = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) != cudaSuccess || !sym)
+            return PICKLE_ERR_DEVICE;
+        fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
+        encode.store(fn, std::memory_order_release);
+    }
+    const cuuint64_t rows = (cuuint64_t)p->n_pages * p->n_kv_heads * (p->page_size / CELL) * 2 * CELL;
+    const cuuint64_t dims[2] = {(cuuint64_t)p->head_dim, rows}, strides[1] = {(cuuint64_t)p->head_dim * 2};
+    const cuuint32_t box[2] = {64, CELL}, one[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p->pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? PICKLE_OK
+               : PICKLE_ERR_DEVICE;
+}
+
 // CTAs per token: enough to fill the SMs when there are few tokens.
 int ctas_per_token(int n_tok, int units, int units_per_cta) {
     const int most = (units + units_per_cta - 1) / units_per_cta;
@@ -450,7 +487,7 @@ int pickle_cuda_pages_append_dev(const pickle_cuda_pages_t* pages, const pickle_
     const int units = (q ? n_heads : 0) + 2 * HK;
     const dim3 grid(batch->n_tok, ctas_per_token(batch->n_tok, units, APPEND_WARPS * 256 / D));
     return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
-        return launch(pages_append_kernel<kv(), d(), rows()>, grid, 32 * APPEND_WARPS, 0, a, (cudaStream_t)stream);
+        return launch(pages_append_kernel<kv(), d(), rows()>, grid, 32 * APPEND_WARPS, 0, (cudaStream_t)stream, a);
     });
 }
 
@@ -468,7 +505,7 @@ int pickle_cuda_pages_read_dev(const pickle_cuda_pages_t* pages, const pickle_cu
     a.v_stride = v_stride;
     const dim3 grid(batch->n_tok, ctas_per_token(batch->n_tok, 2 * HK, READ_WARPS * 256 / D));
     return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
-        return launch(pages_read_kernel<kv(), d(), rows()>, grid, 32 * READ_WARPS, 0, a, (cudaStream_t)stream);
+        return launch(pages_read_kernel<kv(), d(), rows()>, grid, 32 * READ_WARPS, 0, (cudaStream_t)stream, a);
     });
 }
 
@@ -520,18 +557,20 @@ int pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cu
             using T = DecodeTile<kv(), d()>;
             const auto fn = pages_decode_kernel<kv(), d(), rows()>;
             int e = allow_smem(fn, T::SMEM, few_set);
-            if (e == PICKLE_OK) e = launch(fn, dim3(a.w.n_seqs * HK, p.n_splits), 32 * T::WARPS, T::SMEM, a, st);
+            if (e == PICKLE_OK) e = launch(fn, dim3(a.w.n_seqs * HK, p.n_splits), 32 * T::WARPS, T::SMEM, st, a);
             if (e == PICKLE_OK && p.n_splits > 1)
-                e = launch(pages_merge_kernel<d(), rows(), CELL, 0>, merge_grid, 32 * MERGE_WARPS, 0, a, st);
+                e = launch(pages_merge_kernel<d(), rows(), CELL, 0>, merge_grid, 32 * MERGE_WARPS, 0, st, a);
             return e;
         }
         using T = ChunkTile<kv(), d(), rows()>;
         const auto fn = pages_chunk_kernel<kv(), d(), rows()>;
-        int e = allow_smem(fn, T::SMEM, many_set);
+        alignas(64) CUtensorMap tm;
+        int e = rows_map(&tm, pages);
+        if (e == PICKLE_OK) e = allow_smem(fn, T::SMEM, many_set);
         if (e == PICKLE_OK)
-            e = launch(fn, dim3(a.w.n_seqs * HK, p.blocks, p.n_splits), CHUNK_THREADS, T::SMEM, a, st);
+            e = launch(fn, dim3(a.w.n_seqs * HK, p.blocks, p.n_splits), CHUNK_THREADS, T::SMEM, st, tm, a);
         if (e == PICKLE_OK && p.n_splits > 1)
-            e = launch(pages_merge_kernel<d(), rows(), T::BN, T::ROWS_CTA>, merge_grid, 32 * MERGE_WARPS, 0, a, st);
+            e = launch(pages_merge_kernel<d(), rows(), T::BN, T::ROWS_CTA>, merge_grid, 32 * MERGE_WARPS, 0, st, a);
         return e;
     });
 }

@@ -5,18 +5,20 @@
 // (token, query head of the group) pair, as two 128-row tiles A and B that
 // share every tile of keys; with several pieces a CTA takes one piece of the
 // keys and leaves (maximum, sum, O) for the merge.
-//   warp 13     looks pages up and asks for the rows: BF16 pages with TMA
+//   warp 21     looks pages up and asks for the rows: BF16 pages with TMA
 //               tensor copies of a cell's 16 rows straight into the operands'
 //               layout (128-byte swizzle), 8-bit pages with bulk copies of the
 //               codes into a raw buffer, together with their scales;
-//   warps 8-11  turn a tile's codes into 16-bit operands (K-major K, MN-major V);
+//   warps 16-19 turn a tile's codes into 16-bit operands (K-major K, MN-major V);
 //               of BF16 pages they only clear V rows that no row sees;
-//   warp 12     one lane issues tcgen05.mma: S_X = Q_X K^T, O_X += P_X V,
+//   warp 20     one lane issues tcgen05.mma: S_X = Q_X K^T, O_X += P_X V,
 //               P_X read from TMEM, in the order PV_A, S_A, PV_B, S_B so that one
 //               tile's softmax runs under the other's products;
-//   warps 0-3, 4-7  softmax of tile A, B: a thread owns a row. It masks, keeps
-//               the running maximum (O is rescaled only when it grows by more
-//               than 2^8) and writes P over S.
+//   warps 0-7, 8-15  softmax of tile A, B: two threads share a row, one for each
+//               half of a tile's keys. They mask, keep the running maximum
+//               (which moves only when a score passes it by 2^8: the two
+//               warps of 32 rows vote, and only then read each other's half) and
+//               write P over S.
 // 8-bit codes become F16 numbers code * 2^(e - E), exact but for elements
 // 2^-24 below the reference: K has one E for 32 keys of a tile, which the
 // softmax undoes in the factor it applies anyway;
@@ -55,19 +57,27 @@ struct ChunkTile {
     static constexpr int SMEM_KV = TILES * NP * Q_TILE;
     static constexpr int STAGE = 2 * KV_TILE;
     static constexpr int RAW = BF ? 0 : 2 * BN * D;                                // a tile's codes as they come
-    static constexpr int FIT = (232448 - 1024 - 320 - 512 - SMEM_KV - RAW) / STAGE;
+    static constexpr int AUX = 3072;                                               // barriers and words, below
+    static constexpr int FIT = (232448 - AUX - SMEM_KV - RAW) / STAGE;
     static constexpr int STAGES = FIT >= 4 ? 4 : 2;
     static constexpr int SMEM_RAW = SMEM_KV + STAGES * STAGE;
-    static constexpr int SMEM_BAR = SMEM_RAW + RAW;
-    static constexpr int SMEM = SMEM_BAR + 320 + 1024;                             // barriers; alignment (512: static words)
+    static constexpr int SMEM_AUX = SMEM_RAW + RAW;
+    static constexpr int SMEM = SMEM_AUX + AUX;                                    // from a 1024-byte boundary on
     static_assert(FIT >= 2, "the ring needs two stages");
-    static_assert(STAGES * STAGE >= 8 * 4096, "the epilogue's staging reuses the ring");
+    static_assert(STAGES * STAGE >= 16 * 4096, "the epilogue's staging reuses the ring");
 };
 
-constexpr int CHUNK_THREADS = 512;
-constexpr int CHUNK_STAGE_WARP = 8, CHUNK_MMA_WARP = 12, CHUNK_LOAD_WARP = 13;
-// Registers a thread after the split: 8 softmax, 4 staging, 4 other warps; 32 * (8 * 144 + 4 * 104 + 4 * 120) = 65536,
-// what 512 threads of 128 were launched with.
+constexpr int CHUNK_THREADS = 768;
+constexpr int CHUNK_STAGE_WARP = 16, CHUNK_MMA_WARP = 20, CHUNK_LOAD_WARP = 21;
+// Registers a thread after the split: 16 softmax, 4 staging, 4 other warps; 32 * (16 * 80 + 4 * 72 + 4 * 88) = 61440, what
+// 768 threads of 80 were launched with.
+// Barrier `id` of 64 threads; whether any of them says so.
+PCU_DEV bool bar_any(int id, bool x) {
+    uint32_t y;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(y) : "r"(id), "r"((uint32_t)x) : "memory");
+    return y != 0;
+}
 // The lowest n bits, n of any size or sign.
 PCU_DEV uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 PCU_DEV void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
@@ -142,15 +152,27 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     // while the softmax of that S still runs.
     constexpr int INFO = 4 * STAGES;
     constexpr int NCT = BN / CELL;                 // cells of a tile
-    extern __shared__ unsigned char smem_raw[];
+    extern __shared__ __align__(1024) unsigned char base[];
     // Of a tile: K's reference exponents (a quarter of the keys each), V's (a byte per 32 elements), the keys of each cell
     // that some row sees (bit 16: and that lie on a bad page), whether there are any of those. Scales: the tile's
-    // scale bytes, a word a key.
-    __shared__ uint32_t s_km[INFO][4], s_vref[INFO], s_need[INFO][NCT];
-    __shared__ int s_bad[INFO];
-    __shared__ uint32_t s_scale[BF ? 1 : 2][BF ? 1 : BN], s_twin_vref;
-    __shared__ int s_abort;
-    __shared__ uint32_t s_tmem;
+    // scale bytes, a word a key. qexp: what a row of q was scaled by, as an exponent.
+    struct Aux {
+        uint64_t bars[N_BARS];
+        uint32_t km[INFO][4], vref[INFO], need[INFO][NCT];
+        int bad[INFO];
+        uint32_t scale[BF ? 1 : 2][BF ? 4 : BN];
+        unsigned char qexp[256];
+        uint32_t tmem, twin_vref;
+        int abort;
+    };
+    static_assert(sizeof(Aux) <= T::AUX, "the words behind the operands");
+    Aux& aux = *reinterpret_cast<Aux*>(base + T::SMEM_AUX);
+    auto& s_km = aux.km;
+    auto& s_vref = aux.vref;
+    auto& s_need = aux.need;
+    auto& s_bad = aux.bad;
+    auto& s_scale = aux.scale;
+    int& s_abort = aux.abort;
 
     const View& w = a.w;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -176,18 +198,17 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     const int n_all = twin ? n_tiles : max(n_a, n_b);
     auto tile_of = [&](int x, int i) { return twin ? 2 * i + x : i; };      // tile x's i-th tile of keys
 
-    const uint32_t raw_u32 = smem_u32(smem_raw);
-    const uint32_t base_u32 = (raw_u32 + 1023u) & ~1023u;
-    unsigned char* base = smem_raw + (base_u32 - raw_u32);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(base + T::SMEM_BAR);
-    // Twin tiles, in the place of tile B's q: the rows' factors for B, and B's maxima and sums.
-    float* s_rf = reinterpret_cast<float*>(base + NP * T::Q_TILE);
-    float2* s_twin = reinterpret_cast<float2*>(base + NP * T::Q_TILE + 512);
+    const uint32_t base_u32 = smem_u32(base);
+    if (base_u32 & 1023u) {                        // the operands' swizzle goes by address bits
+        record_error(w.err, PCU_DEVERR_ARG);
+        return;
+    }
+    uint64_t* bars = aux.bars;
     if (tid == 0) {
         for (int x = 0; x < 2; ++x) {
-            mbar_init(&bars[Q_FULL + x], 4);
+            mbar_init(&bars[Q_FULL + x], 8);
             mbar_init(&bars[S_FULL + x], 2);      // the products, and the thread that saw the tile's words
-            mbar_init(&bars[P_LO + x], 4);
+            mbar_init(&bars[P_LO + x], 8);       // O rescaled by both halves' warps, and the first half's P
             mbar_init(&bars[P_HI + x], 4);
             mbar_init(&bars[O_DONE + x], 1);
         }
@@ -203,16 +224,16 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         mbar_fence_init();
         s_abort = 0;
     }
-    if (warp == CHUNK_MMA_WARP) tmem_alloc(&s_tmem, 512);
+    if (warp == CHUNK_MMA_WARP) tmem_alloc(&aux.tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = aux.tmem;
     auto aborted = [&]() { return *(volatile int*)&s_abort != 0; };
     auto fail = [&](int code) { record_error(w.err, code); *(volatile int*)&s_abort = 1; };
 
     if (warp >= CHUNK_MMA_WARP) {
-        regs_down<120>();
+        regs_up<88>();
         if (warp == CHUNK_MMA_WARP) {
           if (lane == 0) {
             // ---------------- MMA issue ----------------
@@ -439,7 +460,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             }
         }
     } else if (warp >= CHUNK_STAGE_WARP) {
-        regs_down<104>();
+        regs_down<72>();
         // ---------------- codes -> operands ----------------
         constexpr int KPW = BN / 4;                                 // keys of a tile that this warp turns over
         const int sw = warp - CHUNK_STAGE_WARP;
@@ -533,48 +554,42 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         }
         if (!ok && lane == 0) fail(PCU_DEVERR_EMPTY_WAIT);
     } else {
-        regs_up<144>();
-        // ---------------- softmax: one thread per row of tile X ----------------
-        const int x = warp >> 2, row = (warp & 3) * 32 + lane;
+        // ---------------- softmax: two threads per row of tile X, one for each half of the keys ----------------
+        const int x = warp >> 3, hf = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_tm = tmem + x * 128 + lane_off, o_tm = tmem + 256 + x * D + lane_off;
         const int n_x = x ? n_b : n_a;
         const int xr = twin ? 0 : x;                               // tile of rows
         const int r = cw.r0 + xr * 128 + row;                      // row of the sequence's KV head
         const bool live = r < cw.R && (xr == 0 || has_b);
-        const int tok = r / a.G, head = hk * a.G + r % a.G;
+        const int tok = div_group(r, a), head = hk * a.G + r - tok * a.G;
         const int p = live ? cw.pos0 + tok : -1;
         bool ok = true;
-        float rf = a.scale_log2;
         if (n_x > 0 && x == xr) {
-            // The warp's 32 q rows into shared memory, in the operand order: D / 8 lanes a row, four steps in flight.
-            constexpr int LPR = D / 8, RPS = 32 / LPR, STEPS = 32 / RPS;
-            const int i0 = 8 * (lane % LPR), wr0 = cw.r0 + x * 128 + (warp & 3) * 32;
-            float my_qs = 1.f;
+            // 16 of the tile's q rows a warp into shared memory, in the operand order: D / 8 lanes a row.
+            constexpr int LPR = D / 8, RPS = 32 / LPR, STEPS = 16 / RPS;
+            const int i0 = 8 * (lane % LPR), tr0 = (warp & 7) * 16;
             #pragma unroll 1
             for (int s0 = 0; s0 < STEPS; s0 += 4) {
                 Row8 v[4];
                 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int q = wr0 + (s0 + k) * RPS + lane / LPR;
+                    const int q = cw.r0 + x * 128 + tr0 + (s0 + k) * RPS + lane / LPR, t = div_group(q, a);
                     v[k].a = v[k].b = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (q < cw.R)
-                    {
-                        const int t = div_group(q, a);
                         v[k] = load_row8<ROWS>(a.q, (size_t)(cw.row0 + t) * a.q_stride + (size_t)(hk * a.G + q - t * a.G) * D + i0);
-                    }
                 }
                 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int rr = (s0 + k) * RPS + lane / LPR;              // row of the warp
+                    const int r_t = tr0 + (s0 + k) * RPS + lane / LPR;            // row of the tile
                     float qs = 1.f;
                     if (!BF) {
                         uint32_t m = max(amax_bits(v[k].a), amax_bits(v[k].b));
                         #pragma unroll
                         for (int y = 1; y < LPR; y <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, y));
-                        qs = __uint_as_float(min(268u - (m >> 23), 254u) << 23);
-                        const float theirs = __shfl_sync(0xffffffffu, qs, (lane % RPS) * LPR);
-                        if (lane / RPS == s0 + k) my_qs = theirs;
+                        const uint32_t e = min(268u - (m >> 23), 254u);
+                        qs = __uint_as_float(e << 23);
+                        if (lane % LPR == 0) aux.qexp[x * 128 + r_t] = (unsigned char)e;
                     }
                     const float e[8] = {v[k].a.x * qs, v[k].a.y * qs, v[k].a.z * qs, v[k].a.w * qs,
                                         v[k].b.x * qs, v[k].b.y * qs, v[k].b.z * qs, v[k].b.w * qs};
@@ -584,14 +599,12 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                     split_parts<BF, NP>(e[o2], e[3], q1);
                     split_parts<BF, NP>(e[4], e[4 + o1], q2);
                     split_parts<BF, NP>(e[4 + o2], e[7], q3);
-                    const int c = operand_pos<KV, D>(i0) >> 3, r_t = (warp & 3) * 32 + rr;      // 16-byte chunk, row of the tile
+                    const int c = operand_pos<KV, D>(i0) >> 3;                   // 16-byte chunk of the row
                     const uint32_t to = base_u32 + x * NP * T::Q_TILE + (c >> 3) * T::Q_HALF + r_t * 128 + (((c & 7) ^ (r_t & 7)) << 4);
                     #pragma unroll
                     for (int y = 0; y < NP; ++y) sts128(to + y * T::Q_TILE, make_uint4(q0[y], q1[y], q2[y], q3[y]));
                 }
             }
-            rf = a.scale_log2 / my_qs;
-            if (twin) s_rf[row] = rf;
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars[Q_FULL + x]);
@@ -599,21 +612,21 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         // Positions of the tile's first and last rows: tiles of keys that all of them see need no mask.
         const int p_first = cw.pos0 + (cw.r0 + xr * 128) / a.G;
         const int p_last = cw.pos0 + min(cw.R - 1, cw.r0 + xr * 128 + 127) / a.G;
-        float m_run = -INFINITY, l_run = 0.f;
+        // The two warps of 32 rows: barrier 1 + 4 x + quadrant.
+        const int pair = 1 + x * 4 + (warp & 3);
+        float m_run = -INFINITY, l_run = 0.f, rf = a.scale_log2;
         uint32_t vref = 0;                     // V's references that O is relative to
         for (int i = 0; i < n_x; ++i) {
             const int s = tile_of(x, i) % INFO;
             ok = __all_sync(0xffffffffu, mbar_wait(&bars[S_FULL + x], i & 1));
-            if (!ok) break;
             tc_fence_after();
-            if (i == 0 && x != xr) rf = s_rf[row];           // its products waited for q
+            if (!BF && i == 0) rf = a.scale_log2 / __uint_as_float((uint32_t)aux.qexp[xr * 128 + row] << 23);
             const int j0 = cw.span.step(t0 + tile_of(x, i)) * BN;
             const bool bad = *(volatile int*)&s_bad[s] != 0;
             const bool masked = j0 + BN - 1 > p_first ||
                                 (a.window > 0 && j0 <= p_last - a.window && j0 + BN - 1 >= a.sinks) || bad;
             // Columns [c0, c0 + 32) of the row's scores, those that it does not see as -inf. S is read twice, for the
-            // maximum and for P, 32 columns at a time: short loops stay in the instruction cache next to the
-            // staging's code, which straight-line code for a whole row pushes out once a tile.
+            // maximum and for P, 32 columns at a time: registers and code stay small.
             auto scores = [&](int c0, float (&sc)[32]) {
                 tmem_ld32(s_tm + c0, sc);
                 if (masked) {
@@ -634,69 +647,82 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                 return BF ? rf : fmaxf(rf * (e == 255u ? INFINITY : __uint_as_float(e << 23)), 1.2e-38f);
             };
             constexpr int QN = BN / 4 < 32 ? BN / 4 : 32;             // columns under one factor
-            float m_tile = -INFINITY;
-            #pragma unroll 1
-            for (int c0 = 0; c0 < BN; c0 += 32) {
-                float sc[32];
-                scores(c0, sc);
-                #pragma unroll
-                for (int k = 0; k < 32; k += QN) {
-                    float a0 = sc[k], a1 = sc[k + 1];
+            auto half_max = [&](int h) {
+                float m = -INFINITY;
+                #pragma unroll 1
+                for (int c0 = h * (BN / 2); c0 < (h + 1) * (BN / 2); c0 += 32) {
+                    float sc[32];
+                    scores(c0, sc);
                     #pragma unroll
-                    for (int c = 2; c < QN - 2; c += 4) {
-                        a0 = fmax3(a0, sc[k + c], sc[k + c + 1]);
-                        a1 = fmax3(a1, sc[k + c + 2], sc[k + c + 3]);
+                    for (int k = 0; k < 32; k += QN) {
+                        float a0 = sc[k], a1 = sc[k + 1];
+                        #pragma unroll
+                        for (int c = 2; c < QN - 2; c += 4) {
+                            a0 = fmax3(a0, sc[k + c], sc[k + c + 1]);
+                            a1 = fmax3(a1, sc[k + c + 2], sc[k + c + 3]);
+                        }
+                        m = fmaxf(m, fmax3(fmaxf(a0, a1), sc[k + QN - 2], sc[k + QN - 1]) * factor((c0 + k) / (BN / 4)));
                     }
-                    m_tile = fmaxf(m_tile, fmax3(fmaxf(a0, a1), sc[k + QN - 2], sc[k + QN - 1]) * factor((c0 + k) / (BN / 4)));
                 }
-            }
-            const bool grow = m_tile > m_run + GROW;
+                return m;
+            };
+            // Both halves' S is read before either's P is written over it.
+            float m_tile = half_max(hf);
             float alpha = 1.0f;
-            if (grow) {
-                alpha = ex2(m_run - m_tile);
-                m_run = m_tile;
+            bool grow = false;
+            if (bar_any(pair, m_tile > m_run + GROW || !ok)) {
+                m_tile = fmaxf(m_tile, half_max(hf ^ 1));
+                grow = m_tile > m_run + GROW;
+                if (grow) {
+                    alpha = ex2(m_run - m_tile);
+                    m_run = m_tile;
+                }
+                // Either warp's give-up ends both.
+                if (bar_any(pair, !ok)) {
+                    ok = false;
+                    break;
+                }
             }
             const float nm = m_run == -INFINITY ? 0.f : P_SHIFT - m_run;
             const uint32_t vnow = BF ? 0u : s_vref[s];
+            if (i > 0 && __any_sync(0xffffffffu, grow || vnow != vref)) {
+                // This half's columns of O. S_FULL_X(i) implies PV_X(i - 1) is complete, and PV_X(i) waits for P_LO.
+                #pragma unroll 1
+                for (int c = hf * (D / 64); c < (hf + 1) * (D / 64); ++c) {
+                    float o[32];
+                    tmem_ld32(o_tm + c * 32, o);
+                    const float g = BF ? alpha : alpha * rel_scale((vref >> (8 * c)) & 255, (vnow >> (8 * c)) & 255);
+                    #pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] *= g;
+                    tmem_st32(o_tm + c * 32, o);
+                }
+            }
             float2 sm2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             #pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-                #pragma unroll 1
-                for (int q = 0; q < BN / 64; ++q) {
-                    const int c0 = h * (BN / 2) + q * 32;
-                    float sc[32];
-                    scores(c0, sc);
-                    uint32_t pk[NP][16];
+            for (int c0 = hf * (BN / 2); c0 < (hf + 1) * (BN / 2); c0 += 32) {
+                float sc[32];
+                scores(c0, sc);
+                uint32_t pk[NP][16];
+                #pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    const float ff = factor((c0 + c / QN * QN) / (BN / 4));
+                    const float2 e = ffma2(make_float2(sc[c], sc[c + 1]), make_float2(ff, ff), make_float2(nm, nm));
+                    const float2 pp = make_float2(ex2(e.x), ex2(e.y));
+                    sm2[(c >> 1) & 1] = fadd2(sm2[(c >> 1) & 1], pp);
+                    uint32_t parts[NP];
+                    split_parts<BF, NP>(pp.x, pp.y, parts);
                     #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const float ff = factor((c0 + c / QN * QN) / (BN / 4));
-                        const float2 e = ffma2(make_float2(sc[c], sc[c + 1]), make_float2(ff, ff), make_float2(nm, nm));
-                        const float2 pp = make_float2(ex2(e.x), ex2(e.y));
-                        sm2[(c >> 1) & 1] = fadd2(sm2[(c >> 1) & 1], pp);
-                        uint32_t parts[NP];
-                        split_parts<BF, NP>(pp.x, pp.y, parts);
-                        #pragma unroll
-                        for (int k = 0; k < NP; ++k) pk[k][c >> 1] = parts[k];
-                    }
-                    #pragma unroll
-                    for (int k = 0; k < NP; ++k) tmem_st16(tmem + lane_off + p_column<BN, NP>(x, c0 / 16, k), pk[k]);
+                    for (int k = 0; k < NP; ++k) pk[k][c >> 1] = parts[k];
                 }
-                if (h == 0 && i > 0 && __any_sync(0xffffffffu, grow || vnow != vref)) {
-                    // S_FULL_X(i) implies PV_X(i - 1) is complete, and PV_X(i) waits for the arrival below.
-                    #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        float o[32];
-                        tmem_ld32(o_tm + c * 32, o);
-                        const float g = BF ? alpha : alpha * rel_scale((vref >> (8 * c)) & 255, (vnow >> (8 * c)) & 255);
-                        #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] *= g;
-                        tmem_st32(o_tm + c * 32, o);
-                    }
-                }
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars[(h ? P_HI : P_LO) + x]);
+                #pragma unroll
+                for (int k = 0; k < NP; ++k) tmem_st16(tmem + lane_off + p_column<BN, NP>(x, c0 / 16, k), pk[k]);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&bars[P_LO + x]);
+                if (hf) mbar_arrive(&bars[P_HI + x]);
             }
             const float2 t = fadd2(sm2[0], sm2[1]);
             l_run = l_run * alpha + (t.x + t.y);
@@ -707,55 +733,36 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         if (ok && n_a > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars[O_DONE + 0], 0));
         if (ok && n_b > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars[O_DONE + 1], 0));
         ok = __all_sync(0xffffffffu, ok && !aborted());
-        // Twins: B leaves its statistics, A joins both. m: largest; f_a, f_b: factors of the two outputs, by 32 elements.
-        float f_a = 1.f, f_b = 0.f;
-        uint32_t vref_b = 0;
-        if (twin) {
-            if (x == 1) {
-                s_twin[row] = make_float2(m_run, l_run);
-                if (tid == 128) s_twin_vref = vref;               // the same for all of B's rows
-            }
-            asm volatile("bar.sync 2, 256;" ::: "memory");
-            if (x == 0) {
-                const float2 ml = s_twin[row];
-                const float M = fmaxf(m_run, ml.x), Mz = M == -INFINITY ? 0.f : M;
-                f_a = ex2(m_run - Mz);
-                f_b = ex2(ml.x - Mz);
-                l_run = l_run * f_a + ml.y * f_b;
-                m_run = M;
-                vref_b = s_twin_vref;
-            }
-        }
+        // Each thread's maximum and sum: [tile][half][row], in the place of q.
+        float2* s_ml = reinterpret_cast<float2*>(base);
+        asm volatile("bar.sync 9, 512;" ::: "memory");             // all 16 warps are past the products
+        if (ok) s_ml[(x * 2 + hf) * 128 + row] = make_float2(m_run, l_run);
+        if (tid == 256) aux.twin_vref = vref;                      // tile B's, the same for all of its rows
+        asm volatile("bar.sync 9, 512;" ::: "memory");
         if (ok && (x == 0 || has_b)) {
             tc_fence_after();
+            l_run += s_ml[(x * 2 + (hf ^ 1)) * 128 + row].y;
+            // Twins: A joins both. f_a, f_b: factors of the two outputs.
+            float f_a = 1.f, f_b = 0.f;
+            const uint32_t vref_b = aux.twin_vref;
+            if (twin) {
+                const float2 b0 = s_ml[2 * 128 + row], b1 = s_ml[3 * 128 + row];
+                const float M = fmaxf(m_run, b0.x), Mz = M == -INFINITY ? 0.f : M;
+                f_a = ex2(m_run - Mz);
+                f_b = ex2(b0.x - Mz);
+                l_run = l_run * f_a + (b0.y + b1.y) * f_b;
+                m_run = M;
+            }
             const bool whole = cw.pieces <= 1;
             const float inv = whole ? 1.0f / (l_run == 0.f ? 1.0f : l_run) : 1.0f;
             const size_t rows = (size_t)w.n_tok * a.H;
-            if (!whole && live)
+            if (!whole && live && hf == 0)
                 *reinterpret_cast<float2*>(a.ws_ml + 2 * (split * rows + (size_t)(cw.row0 + tok) * a.H + head)) = make_float2(m_run, l_run);
             const uint32_t stage = base_u32 + T::SMEM_KV + warp * 4096;
             const int wr0 = cw.r0 + x * 128 + (warp & 3) * 32;         // the warp's first row
-            // 128 bytes a row at a time: 32 floats, or 64 BF16 numbers (two loads of 32 columns).
-            auto store_rows = [&](auto f32, int d0) {
-                #pragma unroll 4
-                for (int i = 0; i < 8; ++i) {
-                    const int rr = 4 * i + (lane >> 3), q = wr0 + rr;
-                    const uint4 v = lds128(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-                    if (q < cw.R) {
-                        const int t = div_group(q, a), tk = cw.row0 + t, hd = hk * a.G + q - t * a.G;
-                        if constexpr (decltype(f32)::value) {
-                            float* to = whole ? reinterpret_cast<float*>(a.out) + (size_t)tk * a.out_stride + hd * D
-                                              : a.ws_o + (split * rows + (size_t)tk * a.H + hd) * D;
-                            *reinterpret_cast<uint4*>(to + d0 + 4 * (lane & 7)) = v;
-                        } else {
-                            __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)tk * a.out_stride + hd * D;
-                            *reinterpret_cast<uint4*>(to + d0 + 8 * (lane & 7)) = v;
-                        }
-                    }
-                }
-            };
+            // 32 columns a time through the warp's stage, 128 bytes a row of floats or 64 of BF16 numbers.
             #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = hf * (D / 64); c < (hf + 1) * (D / 64); ++c) {
                 float o[32];
                 if (n_x > 0) {
                     tmem_ld32(o_tm + c * 32, o);
@@ -780,25 +787,37 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                 // Columns are in the operand order: eights of the upper elements change places, fours may be (0, 2, 1, 3).
                 const int swap = KV != BF16 && D == 128 ? c >> 1 : 0;
                 constexpr int n1 = KV == I8 ? 2 : 1, n2 = KV == I8 ? 1 : 2;          // where elements 1 and 2 of a four lie
-                if (ROWS == PICKLE_CUDA_ROW_F32 || !whole) {
-                    __syncwarp();
+                const bool f32 = ROWS == PICKLE_CUDA_ROW_F32 || !whole;
+                __syncwarp();
+                if (f32) {
                     #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        sts128(stage + lane * 128 + ((((i ^ (swap << 1))) ^ (lane & 7)) << 4),
+                        sts128(stage + lane * 128 + (((i ^ (swap << 1)) ^ (lane & 7)) << 4),
                                make_uint4(__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + n1]), __float_as_uint(o[4 * i + n2]),
                                           __float_as_uint(o[4 * i + 3])));
-                    __syncwarp();
-                    store_rows(std::true_type(), c * 32);
                 } else {
-                    if (c % 2 == 0) __syncwarp();
                     #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        sts128(stage + lane * 128 + ((((c % 2) * 4 + (i ^ swap)) ^ (lane & 7)) << 4),
+                        sts128(stage + lane * 128 + (((i ^ swap) ^ (lane & 7)) << 4),
                                make_uint4(bf16x2(o[8 * i], o[8 * i + n1]), bf16x2(o[8 * i + n2], o[8 * i + 3]),
                                           bf16x2(o[8 * i + 4], o[8 * i + 4 + n1]), bf16x2(o[8 * i + 4 + n2], o[8 * i + 7])));
-                    if (c % 2 == 1) {
-                        __syncwarp();
-                        store_rows(std::false_type(), (c - 1) * 32);
+                }
+                __syncwarp();
+                const int lpr = f32 ? 8 : 4, rps = 32 / lpr;           // lanes a row, rows a step
+                #pragma unroll 4
+                for (int i = 0; i < lpr; ++i) {
+                    const int rr = rps * i + lane / lpr, ch = lane % lpr, q = wr0 + rr;
+                    const uint4 v = lds128(stage + rr * 128 + ((ch ^ (rr & 7)) << 4));
+                    if (q < cw.R) {
+                        const int t = div_group(q, a), tk = cw.row0 + t, hd = hk * a.G + q - t * a.G;
+                        if (f32) {
+                            float* to = whole ? reinterpret_cast<float*>(a.out) + (size_t)tk * a.out_stride + hd * D
+                                              : a.ws_o + (split * rows + (size_t)tk * a.H + hd) * D;
+                            *reinterpret_cast<uint4*>(to + c * 32 + 4 * ch) = v;
+                        } else {
+                            __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(a.out) + (size_t)tk * a.out_stride + hd * D;
+                            *reinterpret_cast<uint4*>(to + c * 32 + 8 * ch) = v;
+                        }
                     }
                 }
             }

@@ -144,7 +144,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     constexpr int NP = T::NP, BN = T::BN, STAGES = T::STAGES, NB = D / 32;
     constexpr float P_SHIFT = BF ? 0.f : 7.f, GROW = 8.f;
     constexpr int SLACK = 7;
-    enum { Q_FULL = 0, S_FULL = 2, P_LO = 4, P_HI = 6, O_DONE = 8, DRAIN = 10, K_FULL = 11, K_EMPTY = K_FULL + STAGES,
+    enum { Q_FULL = 0, S_FULL = 2, P_FULL = 4, O_DONE = 6, DRAIN = 8, K_FULL = 9, K_EMPTY = K_FULL + STAGES,
            V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES, RAW_FULL = V_EMPTY + STAGES, RAW_EMPTY = RAW_FULL + 4,
            N_BARS = RAW_EMPTY + 2 };
     static_assert(N_BARS * 8 <= 320, "barriers");
@@ -208,16 +208,15 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         for (int x = 0; x < 2; ++x) {
             mbar_init(&bars[Q_FULL + x], 8);
             mbar_init(&bars[S_FULL + x], 2);      // the products, and the thread that saw the tile's words
-            mbar_init(&bars[P_LO + x], 8);       // O rescaled by both halves' warps, and the first half's P
-            mbar_init(&bars[P_HI + x], 4);
+            mbar_init(&bars[P_FULL + x], 8);
             mbar_init(&bars[O_DONE + x], 1);
         }
         mbar_init(&bars[DRAIN], 1);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&bars[K_FULL + s], BF ? 1 : 4);       // BF16: the TMA copies themselves
             mbar_init(&bars[V_FULL + s], 4);
-            mbar_init(&bars[K_EMPTY + s], 1);
-            mbar_init(&bars[V_EMPTY + s], 1);
+            mbar_init(&bars[K_EMPTY + s], 2);       // by the softmax of the tiles that read it: see there
+            mbar_init(&bars[V_EMPTY + s], 2);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&bars[RAW_FULL + i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&bars[RAW_EMPTY + i], 4);
@@ -237,7 +236,8 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         if (warp == CHUNK_MMA_WARP) {
           if (lane == 0) {
             // ---------------- MMA issue ----------------
-            // One instance of each product's code: three roles share the instruction cache.
+            // One instance of each product's code. A commit holds the tensor pipe up for about 100 cycles, so only S (and
+            // the last O) has one: the softmax that waits for it passes on that K, and the V before, are free.
             const uint32_t id_s = chunk_idesc(BF, BN, 0), id_o = chunk_idesc(BF, D, 1);
             const uint64_t q_desc = smem_desc(base_u32, 16, 1024), k_desc = smem_desc(base_u32 + T::SMEM_KV, 16, 1024);
             const uint64_t v_desc = smem_desc(base_u32 + T::SMEM_KV + T::KV_TILE, T::KV_HALF, 1024);
@@ -255,26 +255,25 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                 #pragma unroll 1
                 for (int x = 0; x < 2 && ok; ++x) {
                     const int n_x = x ? n_b : n_a;
-                    const bool last_reader = twin || x == 1;          // of a tile of keys, where tile B reads it at all
                     if (i >= 0 && i < n_x) {
                         const int j = tile_of(x, i);
                         const uint64_t vd = v_desc + (((j % STAGES) * T::STAGE) >> 4);
                         wait_tile(V_FULL, v_ready, j);
-                        #pragma unroll 1
-                        for (int h = 0; h < 2 && ok; ++h) {
-                            ok = mbar_wait(&bars[(h ? P_HI : P_LO) + x], i & 1);
-                            if (!ok) break;
-                            tc_fence_after();
-                            #pragma unroll
-                            for (int p = 0; p < NP; ++p)
-                                #pragma unroll
-                                for (int k = 0; k < BN / 32; ++k)
-                                    mma_bf16_ts(tmem + 256 + x * D, tmem + p_column<BN, NP>(x, h * (BN / 32) + k, p),
-                                                vd + ((h * (BN / 32) + k) * 16 * 128 >> 4), id_o, i > 0 || h > 0 || p > 0 || k > 0);
-                        }
+                        ok = ok && mbar_wait(&bars[P_FULL + x], i & 1);
                         if (!ok) break;
+                        tc_fence_after();
+                        #pragma unroll
+                        for (int p = 0; p < NP; ++p)
+                            #pragma unroll
+                            for (int k = 0; k < BN / 16; ++k)
+                                mma_bf16_ts(tmem + 256 + x * D, tmem + p_column<BN, NP>(x, k, p), vd + (k * 16 * 128 >> 4), id_o,
+                                            i > 0 || p > 0 || k > 0);
                         if (i + 1 == n_x) mma_commit(&bars[O_DONE + x]);
-                        if (last_reader || i >= n_b) mma_commit(&bars[V_EMPTY + j % STAGES]);
+                        // Twins: this tile's next S needs the K two tiles on, too late a sign for the V that follows it.
+                        if (twin) {
+                            mma_commit(&bars[V_EMPTY + j % STAGES]);
+                            mbar_arrive(&bars[V_EMPTY + j % STAGES]);
+                        }
                     }
                     if (i + 1 < n_x) {
                         const int j = tile_of(x, i + 1), xq = twin ? 0 : x;
@@ -290,7 +289,6 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                                          kd + (((ks / 4) * T::KV_HALF + (ks % 4) * 32) >> 4), id_s, p > 0 || ks > 0);
                         mma_commit(&bars[S_FULL + x]);
                         mbar_arrive(&bars[S_FULL + x]);
-                        if (last_reader || i + 1 >= n_b) mma_commit(&bars[K_EMPTY + j % STAGES]);
                     }
                 }
             }
@@ -614,12 +612,23 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         const int p_last = cw.pos0 + min(cw.R - 1, cw.r0 + xr * 128 + 127) / a.G;
         // The two warps of 32 rows: barrier 1 + 4 x + quadrant.
         const int pair = 1 + x * 4 + (warp & 3);
+        // A key tile that one tile of rows reads alone is passed on twice.
+        auto pass_on = [&](int bar, int k) {
+            const int j = tile_of(x, k);
+            mbar_arrive(&bars[bar + j % STAGES]);
+            if (twin || k >= (x ? n_a : n_b)) mbar_arrive(&bars[bar + j % STAGES]);
+        };
         float m_run = -INFINITY, l_run = 0.f, rf = a.scale_log2;
         uint32_t vref = 0;                     // V's references that O is relative to
         for (int i = 0; i < n_x; ++i) {
             const int s = tile_of(x, i) % INFO;
             ok = __all_sync(0xffffffffu, mbar_wait(&bars[S_FULL + x], i & 1));
             tc_fence_after();
+            // S(i) is made, so its K is free, and so is the V of tile i - 1, whose products came before.
+            if ((warp & 7) == 0 && lane == 0) {
+                pass_on(K_EMPTY, i);
+                if (i > 0 && !twin) pass_on(V_EMPTY, i - 1);
+            }
             if (!BF && i == 0) rf = a.scale_log2 / __uint_as_float((uint32_t)aux.qexp[xr * 128 + row] << 23);
             const int j0 = cw.span.step(t0 + tile_of(x, i)) * BN;
             const bool bad = *(volatile int*)&s_bad[s] != 0;
@@ -686,7 +695,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             const float nm = m_run == -INFINITY ? 0.f : P_SHIFT - m_run;
             const uint32_t vnow = BF ? 0u : s_vref[s];
             if (i > 0 && __any_sync(0xffffffffu, grow || vnow != vref)) {
-                // This half's columns of O. S_FULL_X(i) implies PV_X(i - 1) is complete, and PV_X(i) waits for P_LO.
+                // This half's columns of O. S_FULL_X(i) implies PV_X(i - 1) is complete, and PV_X(i) waits for P_FULL.
                 #pragma unroll 1
                 for (int c = hf * (D / 64); c < (hf + 1) * (D / 64); ++c) {
                     float o[32];
@@ -721,8 +730,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(&bars[P_LO + x]);
-                if (hf) mbar_arrive(&bars[P_HI + x]);
+                mbar_arrive(&bars[P_FULL + x]);
             }
             const float2 t = fadd2(sm2[0], sm2[1]);
             l_run = l_run * alpha + (t.x + t.y);
@@ -730,8 +738,10 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         }
         // ---------------- epilogue ----------------
         // The ring becomes the output's staging once both tiles' products are done.
-        if (ok && n_a > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars[O_DONE + 0], 0));
-        if (ok && n_b > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars[O_DONE + 1], 0));
+        // This tile of rows may end before the other: its last V goes on as well.
+        if (ok && n_x > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars[O_DONE + x], 0));
+        if (ok && n_x > 0 && !twin && (warp & 7) == 0 && lane == 0) pass_on(V_EMPTY, n_x - 1);
+        if (ok && (x ? n_a : n_b) > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars[O_DONE + (x ^ 1)], 0));
         ok = __all_sync(0xffffffffu, ok && !aborted());
         // Each thread's maximum and sum: [tile][half][row], in the place of q.
         float2* s_ml = reinterpret_cast<float2*>(base);

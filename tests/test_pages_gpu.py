@@ -231,6 +231,14 @@ def test_chunks(kv, rows, D, G, HK, page):
     _check_attn(R.Batch(kv, HK, D, page, kv_len, q_len, 22), G, rows)
 
 
+@pytest.mark.parametrize("kv,D", [("bf16", 64), ("bf16", 128), ("i8", 64), ("i8", 128), ("e4m3", 128)])
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("G,n", [(1, 300), (2, 256), (8, 20), (3, 40)])
+def test_tiles_of_rows_that_end_apart(kv, rows, D, G, n):
+    """Both tiles of rows over long contexts: with few heads a group the first one's keys end tiles before the other's."""
+    _check_attn(R.Batch(kv, 1, D, 32, [1500, 1100], [n, 1], 41), G, rows)
+
+
 @pytest.mark.parametrize("kv,rows,D", [("i8", "f32", 128), ("e4m3", "bf16", 128), ("bf16", "bf16", 64),
                                        ("bf16", "f32", 128), ("i8", "bf16", 64)])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (17, 16), (100, 0), (100, 300), (128, 33),

@@ -5,11 +5,12 @@
 // (token, query head of the group) pair, as two 128-row tiles A and B that
 // share every tile of keys; with several pieces a CTA takes one piece of the
 // keys and leaves (maximum, sum, O) for the merge.
-//   warp 21     looks pages up and asks for the rows: BF16 pages with TMA
+//   warps 21, 22 look pages up and ask for the rows of K and of V: BF16 pages with TMA
 //               tensor copies of a cell's 16 rows straight into the operands'
 //               layout (128-byte swizzle), 8-bit pages with bulk copies of the
-//               codes into a raw buffer, together with their scales;
-//   warps 16-19 turn a tile's codes into 16-bit operands (K-major K, MN-major V);
+//               codes into the place of their operands, and their scales;
+//   warps 16-19 turn a tile's codes in place into 16-bit operands (K-major K,
+//               MN-major V);
 //               of BF16 pages they only clear V rows that no row sees;
 //   warp 20     one lane issues tcgen05.mma: S_X = Q_X K^T, O_X += P_X V,
 //               P_X read from TMEM, in the order PV_A, S_A, PV_B, S_B so that one
@@ -56,13 +57,14 @@ struct ChunkTile {
     static constexpr int KV_HALF = BN * 128, KV_TILE = KV_HALF * (D / 64);
     static constexpr int SMEM_KV = TILES * NP * Q_TILE;
     static constexpr int STAGE = 2 * KV_TILE;
-    static constexpr int RAW = BF ? 0 : 2 * BN * D;                                // a tile's codes as they come
-    static constexpr int AUX = 3072;                                               // barriers and words, below
-    static constexpr int FIT = (232448 - AUX - SMEM_KV - RAW) / STAGE;
+    static constexpr int AUX = BF ? 3072 : 6144;                                  // barriers and words, below
+    static constexpr int FIT = (232448 - AUX - SMEM_KV) / STAGE;
     static constexpr int STAGES = FIT >= 4 ? 4 : 2;
-    static constexpr int SMEM_RAW = SMEM_KV + STAGES * STAGE;
-    static constexpr int SMEM_AUX = SMEM_RAW + RAW;
+    static constexpr int SMEM_AUX = SMEM_KV + STAGES * STAGE;
     static constexpr int SMEM = SMEM_AUX + AUX;                                    // from a 1024-byte boundary on
+    // Codes land where their operands will be: row r's D codes in the upper half of what row r (D = 128) or its cell
+    // (D = 64) becomes, and are turned over in place.
+    PCU_DEV static int raw_at(int r) { return D == 128 ? KV_HALF + r * 128 : r / CELL * (CELL * 128) + CELL * 64 + r % CELL * 64; }
     static_assert(FIT >= 2, "the ring needs two stages");
     static_assert(STAGES * STAGE >= 16 * 4096, "the epilogue's staging reuses the ring");
 };
@@ -145,8 +147,8 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     constexpr float P_SHIFT = BF ? 0.f : 7.f, GROW = 8.f;
     constexpr int SLACK = 7;
     enum { Q_FULL = 0, S_FULL = 2, P_FULL = 4, O_DONE = 6, DRAIN = 8, K_FULL = 9, K_EMPTY = K_FULL + STAGES,
-           V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES, RAW_FULL = V_EMPTY + STAGES, RAW_EMPTY = RAW_FULL + 4,
-           N_BARS = RAW_EMPTY + 2 };
+           V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES, RAW_K = V_EMPTY + STAGES, RAW_V = RAW_K + STAGES,
+           N_BARS = RAW_V + STAGES };
     static_assert(N_BARS * 8 <= 320, "barriers");
     // What the loading warp tells the others of a tile outlives the tile's K: K's stage is free once its S is made,
     // while the softmax of that S still runs.
@@ -158,9 +160,9 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     // scale bytes, a word a key. qexp: what a row of q was scaled by, as an exponent.
     struct Aux {
         uint64_t bars[N_BARS];
-        uint32_t km[INFO][4], vref[INFO], need[INFO][NCT];
+        uint32_t km[INFO][4], vref[INFO], need[2][INFO][NCT];
         int bad[INFO];
-        uint32_t scale[BF ? 1 : 2][BF ? 4 : BN];
+        uint32_t scale[BF ? 1 : STAGES][2][BF ? 4 : BN];
         unsigned char qexp[256];
         uint32_t tmem, twin_vref;
         int abort;
@@ -217,9 +219,9 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             mbar_init(&bars[V_FULL + s], 4);
             mbar_init(&bars[K_EMPTY + s], 2);       // by the softmax of the tiles that read it: see there
             mbar_init(&bars[V_EMPTY + s], 2);
+            mbar_init(&bars[RAW_K + s], 1);
+            mbar_init(&bars[RAW_V + s], 1);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(&bars[RAW_FULL + i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&bars[RAW_EMPTY + i], 4);
         mbar_fence_init();
         s_abort = 0;
     }
@@ -296,7 +298,8 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             mma_commit(&bars[DRAIN]);
             if (!mbar_wait(&bars[DRAIN], 0)) record_error(w.err, PCU_DEVERR_DRAIN_WAIT);
           }
-        } else if (warp == CHUNK_LOAD_WARP) {
+        } else if (warp <= CHUNK_LOAD_WARP + 1) {
+            const int v = warp - CHUNK_LOAD_WARP;          // K or V: a copy costs its issuer some 80 cycles
             // ---------------- pages -> shared memory ----------------
             // Lane c < NCT looks after cell c of a tile. need: its keys that some row sees; a page id is asked for two
             // tiles before it is used, and the cell's bytes are asked for in L2 a tile before they are copied.
@@ -361,15 +364,15 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                 }
             };
             if (!BF) scales(x0);
-            int issued = 0;                        // half tiles asked for
+            int issued = 0;                        // tiles asked for
             #pragma unroll 1
             for (int j = 0; j < n_all; ++j) {
                 const int i = j % INFO, st = j % STAGES;
-                if (want(x1)) bulk_prefetch_l2(cell_at(x1), cell_bytes(KV, D));
-                const uint32_t wanted = __popc(__ballot_sync(0xffffffffu, want(x0)));
+                if (v && want(x1)) bulk_prefetch_l2(cell_at(x1), cell_bytes(KV, D));
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, want(x0))) * CELL * D * elem_bytes(KV);
                 const int bad = __any_sync(0xffffffffu, x0.need >> 16);
                 uint32_t km[BN / 32], vm = 0;
-                if (!BF) {
+                if (!BF && v == 0) {
                     // K: one reference for 32 keys. V: a reference moves where the tile's largest exponent passes it by
                     // more than the slack.
                     #pragma unroll
@@ -389,17 +392,15 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                         vm |= (m > old + SLACK ? m : old) << (8 * k);
                     }
                     ev = vm;
-                    if (j > 0) wait(RAW_EMPTY + 0, j - 1);
-                } else if (j >= STAGES) {
-                    wait(K_EMPTY + st, j / STAGES - 1);
                 }
+                if (j >= STAGES) wait((v ? V_EMPTY : K_EMPTY) + st, j / STAGES - 1);
                 if (!ok) break;
-                if (lane < NCT) s_need[i][lane] = x0.need;
+                if (lane < NCT) s_need[v][i][lane] = x0.need;
                 if (!BF) {
                     #pragma unroll
-                    for (int q = 0; q < BN / 32; ++q) s_scale[0][32 * q + lane] = ks[q];
+                    for (int q = 0; q < BN / 32; ++q) s_scale[st][v][32 * q + lane] = v ? vs[q] : ks[q];
                 }
-                if (lane == 0) {
+                if (v == 0 && lane == 0) {
                     s_bad[i] = bad;
                     if (!BF) {
                         s_vref[i] = ev;
@@ -407,53 +408,32 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                         for (int k = 0; k < 4; ++k) s_km[i][k] = km[k * (BN / 32) / 4];
                     }
                 }
+                // BF16: two boxes of 64 columns and 16 rows for each of a cell's K and V. 8-bit: a cell's codes, where
+                // staging turns them over.
+                const uint32_t dst = base_u32 + T::SMEM_KV + st * T::STAGE + v * T::KV_TILE + (BF ? lane * CELL * 128 : T::raw_at(lane * CELL));
+                uint64_t* bar = &bars[(v ? RAW_V : BF ? K_FULL : RAW_K) + st];
                 __syncwarp();
-                if constexpr (BF) {
-                    // Two boxes of 64 columns and 16 rows for each of a cell's K and V.
-                    const uint32_t dst = base_u32 + T::SMEM_KV + st * T::STAGE + lane * CELL * 128;
-                    if (lane == 0) mbar_arrive_expect_tx(&bars[K_FULL + st], wanted * CELL * D * 2);
-                    __syncwarp();
-                    if (want(x0))
+                if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+                __syncwarp();
+                if (want(x0)) {
+                    if constexpr (BF) {
                         for (int h = 0; h < D / 64; ++h)
-                            tma_load_2d(dst + h * T::KV_HALF, &tm, 64 * h, (int)(x0.at * 2 * CELL), &bars[K_FULL + st]);
-                    ++issued;
-                    if (j >= STAGES) wait(V_EMPTY + st, j / STAGES - 1);
-                    if (!ok) break;
-                    if (lane == 0) mbar_arrive_expect_tx(&bars[RAW_FULL + st], wanted * CELL * D * 2);
-                    __syncwarp();
-                    if (want(x0))
-                        for (int h = 0; h < D / 64; ++h)
-                            tma_load_2d(dst + T::KV_TILE + h * T::KV_HALF, &tm, 64 * h, (int)(x0.at * 2 * CELL + CELL), &bars[RAW_FULL + st]);
-                    ++issued;
-                } else {
-                    const uint32_t dst = base_u32 + T::SMEM_RAW + lane * CELL * D;
-                    if (lane == 0) mbar_arrive_expect_tx(&bars[RAW_FULL + 0], wanted * CELL * D);
-                    __syncwarp();
-                    if (want(x0)) bulk_g2s_at(dst, cell_at(x0), CELL * D, &bars[RAW_FULL + 0]);
-                    ++issued;
-                    if (j > 0) wait(RAW_EMPTY + 1, j - 1);
-                    if (!ok) break;
-                    #pragma unroll
-                    for (int q = 0; q < BN / 32; ++q) s_scale[1][32 * q + lane] = vs[q];
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_expect_tx(&bars[RAW_FULL + 1], wanted * CELL * D);
-                    __syncwarp();
-                    if (want(x0)) bulk_g2s_at(dst + BN * D, cell_at(x0) + v_row(KV, D, 0), CELL * D, &bars[RAW_FULL + 1]);
-                    ++issued;
-                    scales(x1);
+                            tma_load_2d(dst + h * T::KV_HALF, &tm, 64 * h, (int)(x0.at * 2 * CELL + v * CELL), bar);
+                    } else {
+                        bulk_g2s_at(dst, cell_at(x0) + (v ? v_row(KV, D, 0) : 0), CELL * D, bar);
+                    }
                 }
+                ++issued;
+                if (!BF) scales(x1);
                 x0 = x1;
                 x1 = look(far, id2);
                 far = ask(j + 3, id2);
             }
             if (!ok || aborted()) {
                 // What was asked for must land before shared memory goes away: the last STAGES tiles cover it.
-                for (int h = max(0, issued - 2 * STAGES); h < issued; ++h) {
-                    const int j = h >> 1, v = h & 1;
-                    const int bar = BF ? (v ? RAW_FULL : K_FULL) + j % STAGES : RAW_FULL + v;
-                    if (h + (BF ? 2 * STAGES : 2) >= issued && !mbar_wait(&bars[bar], (BF ? j / STAGES : j) & 1) && lane == 0)
+                for (int j = max(0, issued - STAGES); j < issued; ++j)
+                    if (!mbar_wait(&bars[(v ? RAW_V : BF ? K_FULL : RAW_K) + j % STAGES], (j / STAGES) & 1) && lane == 0)
                         record_error(w.err, PCU_DEVERR_DRAIN_WAIT);
-                }
                 if (!ok && lane == 0) fail(PCU_DEVERR_EMPTY_WAIT);
             }
         }
@@ -470,15 +450,15 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             if (lane == 0) mbar_arrive(&bars[bar + j % STAGES]);
         };
         // The keys of row r's cell that some row sees, of tile j.
-        auto need_of = [&](int j, int r) { return s_need[j % INFO][r / CELL]; };
+        auto need_of = [&](int v, int j, int r) { return s_need[v][j % INFO][r / CELL]; };
         if constexpr (BF) {
             for (int j = 0; j < n_all; ++j) {
-                wait(RAW_FULL + j % STAGES, j / STAGES);
+                wait(RAW_V + j % STAGES, j / STAGES);
                 if (!ok) break;
                 // Rows that no row of the call sees may hold anything, and 0 times a NaN is no 0: a lane a row.
                 if (lane < KPW) {
                     const int r = sw * KPW + lane;
-                    if (!((need_of(j, r) >> (r % CELL)) & 1)) {
+                    if (!((need_of(1, j, r) >> (r % CELL)) & 1)) {
                         #pragma unroll
                         for (int i = 0; i < D / 8; ++i)
                             sts128(base_u32 + T::SMEM_KV + (j % STAGES) * T::STAGE + T::KV_TILE + (i >> 3) * T::KV_HALF + r * 128 + (i & 7) * 16,
@@ -495,16 +475,15 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             #pragma unroll 1
             for (int step = 0; step < 2 * n_all; ++step) {
                 const int j = step >> 1, v = step & 1, i = j % INFO;
-                wait(RAW_FULL + v, j);
-                if (j >= STAGES) wait((v ? V_EMPTY : K_EMPTY) + j % STAGES, j / STAGES - 1);
+                wait((v ? RAW_V : RAW_K) + j % STAGES, j / STAGES);
                 if (!ok) break;
-                const uint32_t raw = base_u32 + T::SMEM_RAW + v * BN * D + sw * KPW * D;
-                const uint32_t dst = base_u32 + T::SMEM_KV + (j % STAGES) * T::STAGE + v * T::KV_TILE + (k32 >> 1) * T::KV_HALF;
+                const uint32_t tile = base_u32 + T::SMEM_KV + (j % STAGES) * T::STAGE + v * T::KV_TILE;
+                const uint32_t dst = tile + (k32 >> 1) * T::KV_HALF;
                 const int ref = v ? (int)((s_vref[i] >> (8 * k32)) & 255u) : (int)s_km[i][sw];
-                const unsigned char* sc = reinterpret_cast<const unsigned char*>(&s_scale[v][sw * KPW]) + k32;
+                const unsigned char* sc = reinterpret_cast<const unsigned char*>(&s_scale[j % STAGES][v][sw * KPW]) + k32;
                 bool whole = true;
                 #pragma unroll
-                for (int c = 0; c < KPW / CELL; ++c) whole = whole && (s_need[i][sw * (KPW / CELL) + c] & 0xffffu) == 0xffffu;
+                for (int c = 0; c < KPW / CELL; ++c) whole = whole && (s_need[v][i][sw * (KPW / CELL) + c] & 0xffffu) == 0xffffu;
                 #pragma unroll 1
                 for (int q0 = 0; q0 < NI; q0 += 2) {
                     uint4 x[2][2];
@@ -513,7 +492,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                     #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const int row = (q0 + q) * RPS + row0_l, odd = row & 1;
-                        const uint32_t from = raw + row * D + k32 * 32;
+                        const uint32_t from = tile + T::raw_at(sw * KPW + row) + k32 * 32;
                         x[q][0] = lds128(from + odd * 16);
                         x[q][1] = lds128(from + (odd ^ 1) * 16);
                         const float ff = rel_scale(sc[4 * row], ref);
@@ -525,9 +504,10 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                         #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             const int r = sw * KPW + (q0 + q) * RPS + row0_l;
-                            if (!((need_of(j, r) >> (r % CELL)) & 1)) x[q][0] = x[q][1] = make_uint4(0u, 0u, 0u, 0u);
+                            if (!((need_of(v, j, r) >> (r % CELL)) & 1)) x[q][0] = x[q][1] = make_uint4(0u, 0u, 0u, 0u);
                         }
                     }
+                    __syncwarp();                  // a cell is read before any of it is written over
                     #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const int row = (q0 + q) * RPS + row0_l, r = sw * KPW + row;
@@ -547,7 +527,6 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                     }
                 }
                 full(v ? V_FULL : K_FULL, j);
-                if (lane == 0) mbar_arrive(&bars[RAW_EMPTY + v]);       // after the warp's last read (full() syncs it)
             }
         }
         if (!ok && lane == 0) fail(PCU_DEVERR_EMPTY_WAIT);
@@ -644,7 +623,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                     const int hi = max(p, -1) - j0 - c0, sk = a.sinks - j0 - c0;
                     const int lo = (a.window > 0 ? max(max(p, -1) - a.window, -1) : -1) - j0 - c0;
                     uint32_t see = bits_below(hi + 1) & (~bits_below(lo + 1) | bits_below(sk));
-                    if (bad) see &= (s_need[s][c0 / 16] & 0xffffu) | s_need[s][c0 / 16 + 1] << 16;
+                    if (bad) see &= (s_need[0][s][c0 / 16] & 0xffffu) | s_need[0][s][c0 / 16 + 1] << 16;
                     #pragma unroll
                     for (int c = 0; c < 32; ++c)
                         if (!(see & (1u << c))) sc[c] = -INFINITY;

@@ -62,89 +62,120 @@ PCU_DEV void rotate8(Row8& x, const float4 (&c)[2], const float4 (&s)[2], int pa
                       rot<ONCE>(c[1].z, x.b.z, s[1].z, y.b.z), rot<ONCE>(c[1].w, x.b.w, s[1].w, y.b.w));
 }
 
-constexpr int APPEND_WARPS = 4;
+// Where token t's rows go: its page position, found by the warp that handles the token.
+enum { NOT_OURS = 0, NO_PLACE = 1, PLACED = 2 };   // left alone; zero rows, no page; a page position
+struct Place {
+    int state, pos, r;       // position in the sequence, row in the cell
+    uint32_t cell;           // KV head 0's cell in the pool; head h's is h * (page_size / 16) further
+};
 
-// One CTA column per token (blockIdx.x); its H + 2 HK rows are spread over
-// the warps of gridDim.y CTAs. D / 8 lanes hold a row, 8 elements each, so a
-// scale's 32 elements are 4 lanes and a rotation partner is half / 8 lanes
-// away. The token's sin / cos stay in registers for all its rows.
+PCU_DEV Place place_of(const View& w, int t, int rope_len, int lane) {
+    Place x{NOT_OURS, 0, 0, 0u};
+    const int b = t < w.n_tok ? seq_of_row(w, t, lane) : w.n_seqs;
+    int row0, n, kv;
+    if (b >= w.n_seqs || !seq_bounds(w, b, row0, n, kv)) return x;
+    x.pos = kv - n + (t - row0);
+    x.state = NO_PLACE;
+    if (x.pos < 0) return x;
+    if (x.pos >= rope_len) {
+        record_error(w.err, PCU_DEVERR_ARG);
+        return x;
+    }
+    const uint32_t cpp = w.page_size / CELL, cell = (uint32_t)x.pos / CELL, page = cell / cpp;
+    const int id = w.table[(size_t)b * w.table_stride + page];
+    if ((unsigned)id >= (unsigned)w.n_pages) {
+        record_error(w.err, PCU_DEVERR_ARG);
+        return x;
+    }
+    x.state = PLACED;
+    x.r = x.pos % CELL;
+    x.cell = (uint32_t)id * w.HK * cpp + (cell - page * cpp);
+    return x;
+}
+
+constexpr int ROW_WARPS = 4, ROW_AHEAD = 4;        // warps of a CTA; steps whose loads are in flight together
+
+// A warp takes a token; its H + 2 HK rows are spread over gridDim.y warps. D / 8
+// lanes hold a row, 8 elements each, so a scale's 32 elements are 4 lanes and
+// a rotation partner is half / 8 lanes away. The token's sin / cos stay in
+// registers for all its rows. Bound by HBM: rows in, rotated q and codes out.
+// Finding a token's page takes four dependent loads, so a warp has many rows
+// to go with them (two tokens a warp, looked up together, were slower: 92 us
+// against 75, for want of warps).
 template <int KV, int D, int ROWS>
-__global__ void __launch_bounds__(32 * APPEND_WARPS) pages_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(32 * ROW_WARPS) pages_append_kernel(const AppendArgs a) {
     constexpr int LPR = D / 8, RPW = 32 / LPR;
     const View& w = a.w;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     griddep_wait();
     griddep_launch_dependents();
-    const int t = blockIdx.x;
-    const int b = seq_of_row(w, t, lane);
-    if (b >= w.n_seqs) return;
-    int row0, n, kv;
-    if (!seq_bounds(w, b, row0, n, kv)) return;
-    const int pos = kv - n + (t - row0);
-    bool live = pos >= 0;
-    if (live && a.half > 0 && pos >= a.rope_len) {
-        record_error(w.err, PCU_DEVERR_ARG);
-        live = false;
-    }
-    const int page = live ? page_of(w, b, pos) : -1;
+    const int t = blockIdx.x * ROW_WARPS + warp;
+    const Place p = place_of(w, t, a.half > 0 ? a.rope_len : 0x7fffffff, lane);
+    if (p.state == NOT_OURS) return;
     const int sub = lane / LPR, l = lane % LPR, i0 = 8 * l;
     const int hl = a.half / 8;
-    const bool rotated = l < 2 * hl;
-    const int partner = !rotated ? lane : l < hl ? lane + hl : lane - hl;
+    const bool turns = l < 2 * hl;
+    const int partner = !turns ? lane : l < hl ? lane + hl : lane - hl;
+    const int HK = w.HK, nq = a.q ? a.H : 0, units = nq + 2 * HK, cpp = w.page_size / CELL;
+    const int step = gridDim.y * RPW;
+    const bool live = p.state == PLACED, rotated = live && turns;
     float4 c[2], s[2];
-    if (live && rotated) {
-        const size_t at = (size_t)pos * a.half + (l < hl ? i0 : i0 - a.half);
-        const float4* sp = reinterpret_cast<const float4*>(a.sin_tab + at);
-        const float4* cp = reinterpret_cast<const float4*>(a.cos_tab + at);
+    if (rotated) {
+        const size_t o = (size_t)p.pos * a.half + (l < hl ? i0 : i0 - a.half);
+        const float4* sp = reinterpret_cast<const float4*>(a.sin_tab + o);
+        const float4* cp = reinterpret_cast<const float4*>(a.cos_tab + o);
         const float sg = l < hl ? -1.0f : 1.0f;
         #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            c[i] = cp[i];
-            s[i] = sp[i];
-            s[i] = make_float4(sg * s[i].x, sg * s[i].y, sg * s[i].z, sg * s[i].w);
+        for (int k = 0; k < 2; ++k) {
+            c[k] = cp[k];
+            s[k] = sp[k];
+            s[k] = make_float4(sg * s[k].x, sg * s[k].y, sg * s[k].z, sg * s[k].w);
         }
     }
-    const int HK = w.HK, nq = a.q ? a.H : 0, units = nq + 2 * HK;
-    const int step = gridDim.y * APPEND_WARPS * RPW;
-    for (int u0 = (blockIdx.y * APPEND_WARPS + warp) * RPW; u0 < units; u0 += step) {
-        const int u = u0 + sub;
-        const bool mine = u < units, is_q = u < nq, is_v = u >= nq + HK;
-        const int h = is_q ? u : is_v ? u - nq - HK : u - nq;
-        const void* src = is_q ? a.q : is_v ? a.v : a.k;
-        const size_t stride = is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride;
-        Row8 x;
-        x.a = x.b = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (mine && live) x = load_row8<ROWS>(src, (size_t)t * stride + (size_t)h * D + i0);
-        if (u0 < nq + HK) {          // warp-uniform: some row of this step is a q or k row
-            Row8 y = x;
-            if (u0 + RPW <= nq) {
-                rotate8<false>(y, c, s, partner, live && rotated);
-            } else {
-                rotate8<true>(y, c, s, partner, live && rotated && !is_v);
+    for (int u0 = blockIdx.y * RPW; u0 < units; u0 += ROW_AHEAD * step) {
+        RawRow8<ROWS> rows[ROW_AHEAD];
+        #pragma unroll
+        for (int k = 0; k < ROW_AHEAD; ++k) {
+            const int u = u0 + k * step + sub;
+            const bool is_q = u < nq, is_v = u >= nq + HK;
+            const int h = is_q ? u : is_v ? u - nq - HK : u - nq;
+            rows[k].clear();
+            if (u < units && live)
+                rows[k].load(is_q ? a.q : is_v ? a.v : a.k,
+                                          (size_t)t * (is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) + (size_t)h * D + i0);
+        }
+        #pragma unroll
+        for (int k = 0; k < ROW_AHEAD; ++k) {
+            const int uk = u0 + k * step, u = uk + sub;             // uk: the same for the warp
+            if (uk >= units) break;
+            const bool mine = u < units, is_q = u < nq, is_v = u >= nq + HK;
+            const int h = is_q ? u : is_v ? u - nq - HK : u - nq;
+            Row8 x = rows[k].row();
+            // Only K's codes depend on how the rotation's sum was rounded.
+            if (uk + RPW <= nq) rotate8<false>(x, c, s, partner, rotated);
+            else if (uk < nq + HK) rotate8<true>(x, c, s, partner, rotated && !is_v);
+            if (mine && is_q) {
+                const size_t o = (size_t)t * a.q_out_stride + (size_t)h * D + i0;
+                if (a.q_out_bf16) store_row8<PICKLE_CUDA_ROW_BF16>(a.q_out, o, x);
+                else store_row8<PICKLE_CUDA_ROW_F32>(a.q_out, o, x);
             }
-            x = y;
-        }
-        if (mine && is_q) {
-            const size_t at = (size_t)t * a.q_out_stride + (size_t)h * D + i0;
-            if (a.q_out_bf16) store_row8<PICKLE_CUDA_ROW_BF16>(a.q_out, at, x);
-            else store_row8<PICKLE_CUDA_ROW_F32>(a.q_out, at, x);
-        }
-        uint32_t m = 0;
-        if (KV != BF16) {
-            m = max(amax_bits(x.a), amax_bits(x.b));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        }
-        if (mine && !is_q && page >= 0) {
-            const int p = pos % w.page_size, r = p % CELL;
-            unsigned char* cell = cell_ptr<KV, D>(w, page, h, p);
-            if (KV == BF16) {
-                store_row8<PICKLE_CUDA_ROW_BF16>(cell + (is_v ? v_row(KV, D, r) : k_row(KV, D, r)), i0, x);
-            } else {
-                const uint32_t sc = block_scale<KV>(m);
-                *reinterpret_cast<uint2*>(cell + (is_v ? v_row(KV, D, r) : k_row(KV, D, r)) + i0) =
-                    make_uint2(codes4<KV>(x.a, sc), codes4<KV>(x.b, sc));
-                if (l % 4 == 0) cell[(is_v ? v_scale(D, r) : k_scale(D, r)) + i0 / BLOCK] = (unsigned char)sc;
+            if (uk + RPW <= nq) continue;
+            uint32_t m = 0;
+            if (KV != BF16) {
+                m = max(amax_bits(x.a), amax_bits(x.b));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            }
+            if (mine && !is_q && live) {
+                unsigned char* cell = w.pool + (size_t)(p.cell + (uint32_t)(h * cpp)) * cell_bytes(KV, D);
+                unsigned char* row = cell + (is_v ? v_row(KV, D, p.r) : k_row(KV, D, p.r));
+                if (KV == BF16) {
+                    store_row8<PICKLE_CUDA_ROW_BF16>(row, i0, x);
+                } else {
+                    const uint32_t sc = block_scale<KV>(m);
+                    *reinterpret_cast<uint2*>(row + i0) = make_uint2(codes4<KV>(x.a, sc), codes4<KV>(x.b, sc));
+                    if (l % 4 == 0) cell[(is_v ? v_scale(D, p.r) : k_scale(D, p.r)) + i0 / BLOCK] = (unsigned char)sc;
+                }
             }
         }
     }
@@ -158,45 +189,58 @@ struct ReadArgs {
     size_t k_stride, v_stride;
 };
 
-constexpr int READ_WARPS = 4, READ_AHEAD = 4;
-
-// As the writer: a token per blockIdx.x, D / 8 lanes a row, READ_AHEAD rows
-// in flight per lane.
+// As the writer: a token a warp, D / 8 lanes a row, twice as many steps in
+// flight (their loads are 8 bytes a lane).
 template <int KV, int D, int ROWS>
-__global__ void __launch_bounds__(32 * READ_WARPS) pages_read_kernel(const ReadArgs a) {
-    constexpr int LPR = D / 8, RPW = 32 / LPR;
+__global__ void __launch_bounds__(32 * ROW_WARPS) pages_read_kernel(const ReadArgs a) {
+    constexpr int LPR = D / 8, RPW = 32 / LPR, AHEAD = 2 * ROW_AHEAD;
     const View& w = a.w;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     griddep_wait();
     griddep_launch_dependents();
-    const int t = blockIdx.x;
-    const int b = seq_of_row(w, t, lane);
-    if (b >= w.n_seqs) return;
-    int row0, n, kv;
-    if (!seq_bounds(w, b, row0, n, kv)) return;
-    const int pos = kv - n + (t - row0);
-    const int page = pos >= 0 ? page_of(w, b, pos) : -1;
-    const int p = page >= 0 ? pos % w.page_size : 0, r = p % CELL;
-    const int sub = lane / LPR, i0 = 8 * (lane % LPR), units = 2 * w.HK;
-    const int step = gridDim.y * READ_WARPS * RPW;
-    for (int u0 = (blockIdx.y * READ_WARPS + warp) * RPW + sub; u0 < units; u0 += READ_AHEAD * step) {
-        Row8 x[READ_AHEAD];
+    const int t = blockIdx.x * ROW_WARPS + warp;
+    const Place p = place_of(w, t, 0x7fffffff, lane);
+    if (p.state == NOT_OURS) return;
+    const int sub = lane / LPR, i0 = 8 * (lane % LPR), units = 2 * w.HK, cpp = w.page_size / CELL;
+    const int step = gridDim.y * RPW;
+    for (int u0 = blockIdx.y * RPW + sub; u0 < units; u0 += AHEAD * step) {
+        uint4 raw[AHEAD];
+        uint32_t sc[AHEAD];
         #pragma unroll
-        for (int i = 0; i < READ_AHEAD; ++i) {
-            const int u = u0 + i * step;
-            x[i].a = x[i].b = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (u < units && page >= 0) {
+        for (int k = 0; k < AHEAD; ++k) {
+            const int u = u0 + k * step;
+            raw[k] = make_uint4(0u, 0u, 0u, 0u);
+            sc[k] = 0;
+            if (u < units && p.state == PLACED) {
                 const bool is_v = u >= w.HK;
-                x[i] = load_cached8<KV, D>(cell_ptr<KV, D>(w, page, is_v ? u - w.HK : u, p), r, i0, is_v);
+                const unsigned char* cell = w.pool + (size_t)(p.cell + (uint32_t)((is_v ? u - w.HK : u) * cpp)) * cell_bytes(KV, D);
+                const unsigned char* row = cell + (is_v ? v_row(KV, D, p.r) : k_row(KV, D, p.r));
+                if (KV == BF16) {
+                    raw[k] = *reinterpret_cast<const uint4*>(row + 2 * i0);
+                } else {
+                    const uint2 c = *reinterpret_cast<const uint2*>(row + i0);
+                    raw[k].x = c.x;
+                    raw[k].y = c.y;
+                    sc[k] = cell[(is_v ? v_scale(D, p.r) : k_scale(D, p.r)) + i0 / BLOCK];
+                }
             }
         }
         #pragma unroll
-        for (int i = 0; i < READ_AHEAD; ++i) {
-            const int u = u0 + i * step;
+        for (int k = 0; k < AHEAD; ++k) {
+            const int u = u0 + k * step;
             if (u >= units) break;
             const bool is_v = u >= w.HK;
             const int h = is_v ? u - w.HK : u;
-            store_row8<ROWS>(is_v ? a.v : a.k, (size_t)t * (is_v ? a.v_stride : a.k_stride) + (size_t)h * D + i0, x[i]);
+            Row8 x;
+            if (KV == BF16) {
+                x = bf16_row8(raw[k]);
+            } else {
+                const float f = scale_f32(sc[k]);
+                x = Row8{numbers4<KV>(raw[k].x), numbers4<KV>(raw[k].y)};
+                x.a = make_float4(x.a.x * f, x.a.y * f, x.a.z * f, x.a.w * f);
+                x.b = make_float4(x.b.x * f, x.b.y * f, x.b.z * f, x.b.w * f);
+            }
+            store_row8<ROWS>(is_v ? a.v : a.k, (size_t)t * (is_v ? a.v_stride : a.k_stride) + (size_t)h * D + i0, x);
         }
     }
 }
@@ -436,11 +480,15 @@ int rows_map(CUtensorMap* map, const pickle_cuda_pages_t* p) {
                : PICKLE_ERR_DEVICE;
 }
 
-// CTAs per token: enough to fill the SMs when there are few tokens.
-int ctas_per_token(int n_tok, int units, int units_per_cta) {
-    const int most = (units + units_per_cta - 1) / units_per_cta;
-    const int want = (4 * sm_count() + n_tok - 1) / n_tok;
-    return want < 1 ? 1 : want < most ? want : most;
+// CTAs of ROW_WARPS tokens, and over how many of them a token's `steps` warp
+// steps are spread: about 16 a warp (4 prompts of 2048 tokens with 96 rows:
+// 84, 75, 73 and 82 us at 48, 24, 12 and 6 steps a warp; reading 16 rows back:
+// 38 and 48 us at 8 and 4), fewer where that leaves SMs without work.
+dim3 row_grid(int n_tok, int steps) {
+    const int x = (n_tok + ROW_WARPS - 1) / ROW_WARPS;
+    const int fill = (4 * sm_count() + x - 1) / x, most = (steps + 15) / 16;
+    const int y = fill > most ? fill : most;
+    return dim3(x, y < 1 ? 1 : y < steps ? y : steps);
 }
 
 }  // namespace
@@ -484,10 +532,10 @@ int pickle_cuda_pages_append_dev(const pickle_cuda_pages_t* pages, const pickle_
     a.H = n_heads;
     a.half = half;
     a.rope_len = rope_len;
-    const int units = (q ? n_heads : 0) + 2 * HK;
-    const dim3 grid(batch->n_tok, ctas_per_token(batch->n_tok, units, APPEND_WARPS * 256 / D));
+    const int units = (q ? n_heads : 0) + 2 * HK, rpw = 256 / D;
+    const dim3 grid = row_grid(batch->n_tok, (units + rpw - 1) / rpw);
     return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
-        return launch(pages_append_kernel<kv(), d(), rows()>, grid, 32 * APPEND_WARPS, 0, (cudaStream_t)stream, a);
+        return launch(pages_append_kernel<kv(), d(), rows()>, grid, 32 * ROW_WARPS, 0, (cudaStream_t)stream, a);
     });
 }
 
@@ -503,9 +551,9 @@ int pickle_cuda_pages_read_dev(const pickle_cuda_pages_t* pages, const pickle_cu
     a.v = v_out;
     a.k_stride = k_stride;
     a.v_stride = v_stride;
-    const dim3 grid(batch->n_tok, ctas_per_token(batch->n_tok, 2 * HK, READ_WARPS * 256 / D));
+    const dim3 grid = row_grid(batch->n_tok, (2 * HK * D + 255) / 256);
     return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
-        return launch(pages_read_kernel<kv(), d(), rows()>, grid, 32 * READ_WARPS, 0, (cudaStream_t)stream, a);
+        return launch(pages_read_kernel<kv(), d(), rows()>, grid, 32 * ROW_WARPS, 0, (cudaStream_t)stream, a);
     });
 }
 

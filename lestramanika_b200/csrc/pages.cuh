@@ -35,21 +35,6 @@ struct View {
     int* err;
 };
 
-// Cell of position p of the page (byte offsets pass 2^31 in a large pool).
-template <int KV, int D>
-PCU_DEV unsigned char* cell_ptr(const View& w, int page, int head, int p_in_page) {
-    const size_t cells = (size_t)w.page_size / CELL;
-    return w.pool + (((size_t)page * w.HK + head) * cells + p_in_page / CELL) * cell_bytes(KV, D);
-}
-
-// The page of position p of sequence b, or -1 (recorded) outside the pool.
-PCU_DEV int page_of(const View& w, int b, int p) {
-    const int id = w.table[(size_t)b * w.table_stride + p / w.page_size];
-    if ((unsigned)id < (unsigned)w.n_pages) return id;
-    record_error(w.err, PCU_DEVERR_ARG);
-    return -1;
-}
-
 // The sequence that row t belongs to, found by a whole warp at once: the
 // number of sequences that end at or before t. n_seqs: t is behind the last.
 PCU_DEV int seq_of_row(const View& w, int t, int lane) {
@@ -139,6 +124,15 @@ struct Row8 {
     float4 a, b;
 };
 
+PCU_DEV Row8 bf16_row8(const uint4& u) {
+    Row8 r;
+    r.a = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                      __uint_as_float(u.y & 0xffff0000u));
+    r.b = make_float4(__uint_as_float(u.z << 16), __uint_as_float(u.z & 0xffff0000u), __uint_as_float(u.w << 16),
+                      __uint_as_float(u.w & 0xffff0000u));
+    return r;
+}
+
 template <int ROWS>
 PCU_DEV Row8 load_row8(const void* base, size_t i) {
     Row8 r;
@@ -147,14 +141,35 @@ PCU_DEV Row8 load_row8(const void* base, size_t i) {
         r.a = p[0];
         r.b = p[1];
     } else {
-        const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + i);
-        r.a = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                          __uint_as_float(u.y & 0xffff0000u));
-        r.b = make_float4(__uint_as_float(u.z << 16), __uint_as_float(u.z & 0xffff0000u), __uint_as_float(u.w << 16),
-                          __uint_as_float(u.w & 0xffff0000u));
+        r = bf16_row8(*reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + i));
     }
     return r;
 }
+
+// The same as loaded, not yet turned into F32 (BF16 rows: half the registers).
+template <int ROWS>
+struct RawRow8 {
+    uint4 u[ROWS == PICKLE_CUDA_ROW_F32 ? 2 : 1];
+    PCU_DEV void clear() {
+        #pragma unroll
+        for (auto& x : u) x = make_uint4(0u, 0u, 0u, 0u);
+    }
+    PCU_DEV void load(const void* base, size_t i) {
+        if (ROWS == PICKLE_CUDA_ROW_F32) {
+            const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(base) + i);
+            #pragma unroll
+            for (int k = 0; k < (int)(sizeof(u) / sizeof(u[0])); ++k) u[k] = p[k];
+        } else {
+            u[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(base) + i);
+        }
+    }
+    PCU_DEV Row8 row() const {
+        if (ROWS == PICKLE_CUDA_ROW_BF16) return bf16_row8(u[0]);
+        const uint4 &x = u[0], &y = u[ROWS == PICKLE_CUDA_ROW_F32 ? 1 : 0];
+        return Row8{make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w)),
+                    make_float4(__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w))};
+    }
+};
 
 template <int ROWS>
 PCU_DEV void store_row8(void* base, size_t i, const Row8& r) {
@@ -166,19 +181,6 @@ PCU_DEV void store_row8(void* base, size_t i, const Row8& r) {
         const uint2 lo = pack_bf16x4(r.a, 1.0f), hi = pack_bf16x4(r.b, 1.0f);
         *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(base) + i) = make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
-}
-
-// Eight elements of a cached row from element i on, as F32.
-template <int KV, int D>
-PCU_DEV Row8 load_cached8(const unsigned char* cell, int r, int i, bool is_v) {
-    const unsigned char* row = cell + (is_v ? v_row(KV, D, r) : k_row(KV, D, r));
-    if (KV == BF16) return load_row8<PICKLE_CUDA_ROW_BF16>(row, i);
-    const uint2 c = *reinterpret_cast<const uint2*>(row + i);
-    const float s = scale_f32(cell[(is_v ? v_scale(D, r) : k_scale(D, r)) + i / BLOCK]);
-    Row8 x{numbers4<KV>(c.x), numbers4<KV>(c.y)};
-    x.a = make_float4(x.a.x * s, x.a.y * s, x.a.z * s, x.a.w * s);
-    x.b = make_float4(x.b.x * s, x.b.y * s, x.b.z * s, x.b.w * s);
-    return x;
 }
 
 }  // namespace pages

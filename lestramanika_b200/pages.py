@@ -143,6 +143,7 @@ class KVPages:
         self._refs = [ctypes.byref(c) for c in self._c]
         self._row_types = {torch.float32: ROW_F32, torch.bfloat16: ROW_BF16}
         self._lib = lib()
+        self._layouts = {}
 
     def _tables(self, rope_len, theta, inv_freq, dev):
         # src/pickle_fast.c:1638-1640, 1772-1788: half = min(D/2, 64), inv_freq and angles in F32.
@@ -156,17 +157,31 @@ class KVPages:
     # -- argument checks -------------------------------------------------
     def _rows(self, t, heads, n_tok, what):
         """(address, element type, elements between tokens) of rows [n_tok][heads][D]."""
+        shape = t.shape
+        key = (t.dtype, shape, t.stride(), heads)
+        known = self._layouts.get(key)
+        if known is None:
+            known = self._layout(t, heads, what)
+            if len(self._layouts) >= 1024:
+                self._layouts.clear()
+            self._layouts[key] = known
+        if shape[0] < n_tok or t.get_device() != self.device:
+            raise PickleError(ERR_ARG, "KVPages", f"{what}: fewer rows than the batch's {n_tok}, or not on {self._dev}")
+        return t.data_ptr(), known[0], known[1]
+
+    def _layout(self, t, heads, what):
+        """(element type, elements between tokens) of a tensor's shape and strides, or an error."""
         rt = self._row_types.get(t.dtype)
         shape, st = t.shape, t.stride()
-        if rt is None or t.device != self._dev or len(shape) != 3 or shape[0] < n_tok or shape[2] != self.D or (
-                heads and shape[1] != heads) or st[2] != 1 or (st[1] != self.D and shape[1] > 1):
-            raise PickleError(ERR_ARG, "KVPages", f"{what}: F32 or BF16 rows [n_tok][heads][{self.D}] on {self._dev}, "
-                              "heads and elements dense")
+        if rt is None or len(shape) != 3 or shape[2] != self.D or (heads and shape[1] != heads) or (
+                st[2] != 1 or (st[1] != self.D and shape[1] > 1)):
+            raise PickleError(ERR_ARG, "KVPages", f"{what}: F32 or BF16 rows [n_tok][heads][{self.D}], heads and "
+                              "elements dense")
         if shape[0] <= 1:
-            return t.data_ptr(), rt, 0
+            return rt, 0
         if st[0] < shape[1] * self.D:
             raise PickleError(ERR_ARG, "KVPages", f"{what}: rows overlap")
-        return t.data_ptr(), rt, st[0]
+        return rt, st[0]
 
     def _call(self, batch, layer, stream):
         if not 0 <= layer < self.n_layers or batch.device != self._dev:

@@ -358,24 +358,27 @@ struct Plan {
 };
 
 // How many pieces the keys of `groups` independent streams of `steps` steps
-// are cut into, on `slots` CTA slots: waves of CTAs of the same length. A
-// step takes step_s alone in its slot, or what HBM needs for the wave's
-// bytes; a wave adds a ramp, several pieces add the join and its traffic.
+// are cut into: waves of CTAs of the same length, per_sm of them on an SM. A
+// step takes step_s[k - 1] in a CTA that shares its SM with k - 1 others, or what
+// HBM needs for the wave's bytes; a wave adds a ramp, several pieces add the
+// join (a launch, and a piece at a time) and its traffic.
 struct Costs {
-    double step_s, step_bytes, ramp_s, join_s, join_bytes;
+    int per_sm;
+    double step_s[3], step_bytes, ramp_s, join_s, join_piece_s, join_bytes;
 };
-int plan_pieces(long long groups, long long steps, long long slots, const Costs& c) {
+int plan_pieces(long long groups, long long steps, int sms, const Costs& c) {
     // The same plan is asked for layer after layer, step after step.
     struct Memo {
-        long long groups, steps, slots;
+        long long groups, steps;
+        int sms, pick;
         double a, b;
-        int pick;
     };
     static thread_local Memo memo[16];
     Memo& k = memo[(unsigned long long)(groups * 31 + steps) % 16];
-    if (k.pick && k.groups == groups && k.steps == steps && k.slots == slots && k.a == c.step_s && k.b == c.join_bytes)
+    if (k.pick && k.groups == groups && k.steps == steps && k.sms == sms && k.a == c.step_s[0] && k.b == c.join_bytes)
         return k.pick;
     const double hbm = 6.5e12;
+    const long long slots = (long long)sms * c.per_sm;
     const int most = steps < 64 ? (int)steps : 64;
     double best = 1e30;
     int pick = 1;
@@ -384,17 +387,17 @@ int plan_pieces(long long groups, long long steps, long long slots, const Costs&
         if ((steps + chunk - 1) / chunk != s) continue;
         const long long n = groups * s, full = n / slots, rem = n % slots;
         auto wave = [&](long long ctas) {
-            const double alone = c.step_s * chunk, bytes = c.step_bytes * chunk * ctas / hbm;
+            const double alone = c.step_s[(ctas + sms - 1) / sms - 1] * chunk, bytes = c.step_bytes * chunk * ctas / hbm;
             return (alone > bytes ? alone : bytes) + c.ramp_s;
         };
         double t = full * wave(slots) + (rem ? wave(rem) : 0.0);
-        if (s > 1) t += c.join_s + s * c.join_bytes / hbm;
+        if (s > 1) t += c.join_s + s * (c.join_piece_s + c.join_bytes / hbm);
         if (t < best) {
             best = t;
             pick = s;
         }
     }
-    k = Memo{groups, steps, slots, c.step_s, c.join_bytes, pick};
+    k = Memo{groups, steps, sms, pick, c.step_s[0], c.join_bytes};
     return pick;
 }
 
@@ -431,19 +434,26 @@ Plan plan_attn(const View& w, int kv_type, int D, int row_type, int H, int windo
     Costs c;
     c.step_bytes = bytes;
     c.join_bytes = 2.0 * w.n_tok * H * D * 4;
-    int slots = sm_count();
+    const int sms = sm_count() > 0 ? sm_count() : 1;
     if (p.few) {
-        // One CTA streams at most 33 GB/s.
-        c.step_s = bytes / 33e9;
-        c.ramp_s = 3e-6;
-        c.join_s = 3e-6;
-        slots *= kv_type == BF16 ? 3 : 2;
+        // Fitted to sweeps of the piece count (8B-shaped B = 1, 70B-shaped B = 16, 4096 of 32768 keys in a window): a
+        // CTA streams 33 GB/s (8-bit) or 35 GB/s (BF16) alone on its SM, two 18.5 or 22 each, three BF16 ones 17.
+        c.per_sm = kv_type == BF16 ? 3 : 2;
+        const double rate[2][3] = {{33e9, 18.5e9, 18.5e9}, {35e9, 22e9, 17e9}};
+        for (int k = 0; k < 3; ++k) c.step_s[k] = bytes / rate[kv_type == BF16][k];
+        c.ramp_s = 4e-6;
+        c.join_s = 2.5e-6;
+        c.join_piece_s = 0.1e-6;
     } else {
-        c.step_s = (row_type == PICKLE_CUDA_ROW_F32 ? 2.0e-6 : 1.2e-6) * cd.bn / 128;
-        c.ramp_s = 5e-6;
-        c.join_s = 4e-6;
+        c.per_sm = 1;
+        // A tile of 128 keys takes this long with 256 rows, and two thirds of it with 128 or fewer.
+        const double tile = (row_type != PICKLE_CUDA_ROW_F32 ? 2.5e-6 : D == 64 ? 3.1e-6 : kv_type == BF16 ? 8e-6 : 5e-6) * cd.bn / 128;
+        c.step_s[0] = c.step_s[1] = c.step_s[2] = (long long)w.max_q * G <= 128 ? tile * 0.7 : tile;
+        c.ramp_s = 10e-6;
+        c.join_s = 3e-6;
+        c.join_piece_s = 0.1e-6;
     }
-    p.n_splits = plan_pieces(groups, steps, slots < 1 ? 1 : slots, c);
+    p.n_splits = plan_pieces(groups, steps, sms, c);
     // Knob for sweeps of the piece count.
     if (const char* env = getenv("PICKLE_CUDA_PAGES_SPLITS"))
         if (atoi(env) > 0) p.n_splits = atoi(env) < steps ? atoi(env) : (int)steps;

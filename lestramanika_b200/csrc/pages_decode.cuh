@@ -124,8 +124,13 @@ PCU_DEV uint32_t e4m3x2_f16x2(uint32_t pair) {
     return h;
 }
 
-// Bytes 0 and 2 of x as F16 numbers 1152 + code (the offset-binary code in the low byte of 1024's mantissa).
-PCU_DEV uint32_t i8_magic(uint32_t x) { return (x & 0x00ff00ffu) ^ 0x64806480u; }
+// Bytes 0 and 2 of x as F16 numbers 1152 + code (the offset-binary code in the low byte of 1024's mantissa): one
+// three-input operation, (x & mask) ^ magic, which the compiler makes two of when both constants are literals.
+PCU_DEV uint32_t i8_magic(uint32_t x) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(y) : "r"(x), "r"(0x00ff00ffu), "r"(0x64806480u));
+    return y;
+}
 
 // Four consecutive codes of a row, times f (both halves): the pairs of one k-step. I8: elements (0, 2), (1, 3);
 // E4M3: (0, 1), (2, 3). c = -1152 f; the fused product is exact.

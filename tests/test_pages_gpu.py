@@ -482,3 +482,15 @@ def test_session_of_requests(kv, rows, window, sinks):
     if window:
         assert len(slots.free) + sum(p >= 0 for o in slots.pages.values() for p in o) == 24
         assert any(p < 0 for p in slots.pages["a"])
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[9000] + [1] * 40, [1] * 300, [5000, 0, 4999, 0, 0, 3], [513] * 97, list(range(1, 700, 2))])
+def test_ragged_decodes(rows, lens):
+    """Long sequences next to short ones and unused entries, more sequences than a CTA has threads: the pieces that the
+    longest one is cut into leave the others with empty ones."""
+    B = R.Batch("e4m3", 2, 64, 16, lens, [1] * len(lens), 43)
+    q = B.randn(B.n_tok, 6, 64).to(R.ROWS[rows])
+    first = _check_attn(B, 3, rows, q=q)
+    assert torch.equal(first, _check_attn(B, 3, rows, q=q))             # the same bits again
+    _check_attn(B, 3, rows, 300, 20, q=q)

@@ -361,21 +361,28 @@ struct Plan {
 // are cut into: waves of CTAs of the same length, per_sm of them on an SM. A
 // step takes step_s[k - 1] in a CTA that shares its SM with k - 1 others, or what
 // HBM needs for the wave's bytes; a wave adds a ramp, several pieces add the
-// join (a launch, and a piece at a time) and its traffic.
+// join (a launch, and a piece at a time) and its traffic. The host knows the longest
+// stream only: where streams may differ, what counts is this time plus that
+// of lengths spread evenly from none to `steps`, the work shared out with
+// half a piece's time left over (32 sequences of 8192 keys, 8 heads: one piece 130 us, 8 pieces 72 where they are
+// ragged, up to 6% lost where they are not).
 struct Costs {
     int per_sm;
-    double step_s[3], step_bytes, ramp_s, join_s, join_piece_s, join_bytes;
+    bool ragged;
+    double step_s[4], step_bytes, ramp_s, join_s, join_piece_s, join_bytes;
 };
 int plan_pieces(long long groups, long long steps, int sms, const Costs& c) {
     // The same plan is asked for layer after layer, step after step.
     struct Memo {
         long long groups, steps;
         int sms, pick;
+        bool ragged;
         double a, b;
     };
     static thread_local Memo memo[16];
     Memo& k = memo[(unsigned long long)(groups * 31 + steps) % 16];
-    if (k.pick && k.groups == groups && k.steps == steps && k.sms == sms && k.a == c.step_s[0] && k.b == c.join_bytes)
+    if (k.pick && k.groups == groups && k.steps == steps && k.sms == sms && k.ragged == c.ragged && k.a == c.step_s[0] &&
+        k.b == c.join_bytes)
         return k.pick;
     const double hbm = 6.5e12;
     const long long slots = (long long)sms * c.per_sm;
@@ -385,19 +392,25 @@ int plan_pieces(long long groups, long long steps, int sms, const Costs& c) {
     for (int s = 1; s <= most; ++s) {
         const long long chunk = (steps + s - 1) / s;
         if ((steps + chunk - 1) / chunk != s) continue;
-        const long long n = groups * s, full = n / slots, rem = n % slots;
         auto wave = [&](long long ctas) {
             const double alone = c.step_s[(ctas + sms - 1) / sms - 1] * chunk, bytes = c.step_bytes * chunk * ctas / hbm;
             return (alone > bytes ? alone : bytes) + c.ramp_s;
         };
+        const long long n = groups * s, full = n / slots, rem = n % slots;
         double t = full * wave(slots) + (rem ? wave(rem) : 0.0);
-        if (s > 1) t += c.join_s + s * (c.join_piece_s + c.join_bytes / hbm);
+        if (c.ragged) {
+            const long long some = groups * (s + 1) / 2;
+            const double step = c.step_s[c.per_sm - 1], first = wave(some < 1 ? 1 : some < slots ? some : slots);
+            const double shared = (0.5 * groups * steps * step + some * c.ramp_s) / slots + 0.5 * chunk * step;
+            t += first > shared ? first : shared;
+        }
+        if (s > 1) t += (c.ragged ? 2 : 1) * (c.join_s + s * (c.join_piece_s + c.join_bytes / hbm));
         if (t < best) {
             best = t;
             pick = s;
         }
     }
-    k = Memo{groups, steps, sms, pick, c.step_s[0], c.join_bytes};
+    k = Memo{groups, steps, sms, pick, c.ragged, c.step_s[0], c.join_bytes};
     return pick;
 }
 
@@ -436,19 +449,21 @@ Plan plan_attn(const View& w, int kv_type, int D, int row_type, int H, int windo
     c.join_bytes = 2.0 * w.n_tok * H * D * 4;
     const int sms = sm_count() > 0 ? sm_count() : 1;
     if (p.few) {
-        // Fitted to sweeps of the piece count (8B-shaped B = 1, 70B-shaped B = 16, 4096 of 32768 keys in a window): a
-        // CTA streams 33 GB/s (8-bit) or 35 GB/s (BF16) alone on its SM, two 18.5 or 22 each, three BF16 ones 17.
-        c.per_sm = kv_type == BF16 ? 3 : 2;
-        const double rate[2][3] = {{33e9, 18.5e9, 18.5e9}, {35e9, 22e9, 17e9}};
-        for (int k = 0; k < 3; ++k) c.step_s[k] = bytes / rate[kv_type == BF16][k];
-        c.ramp_s = 4e-6;
+        // Fitted to sweeps of the piece count (1 to 128 sequences of 2048 to 32768 keys, ragged or not): a CTA
+        // streams 19.5 GB/s (8-bit) or 35 GB/s (BF16) alone on its SM, four 9.7 each, three BF16 ones 17.
+        c.per_sm = kv_type == BF16 ? 3 : 4;
+        c.ragged = w.n_seqs > 1 && window == 0;
+        const double rate[2][4] = {{19.5e9, 16e9, 12.3e9, 9.7e9}, {35e9, 22e9, 17e9, 17e9}};
+        for (int k = 0; k < 4; ++k) c.step_s[k] = bytes / rate[kv_type == BF16][k];
+        c.ramp_s = 5e-6;
         c.join_s = 2.5e-6;
         c.join_piece_s = 0.1e-6;
     } else {
         c.per_sm = 1;
+        c.ragged = false;
         // A tile of 128 keys takes this long with 256 rows, and two thirds of it with 128 or fewer.
         const double tile = (row_type != PICKLE_CUDA_ROW_F32 ? 2.5e-6 : D == 64 ? 3.1e-6 : kv_type == BF16 ? 8e-6 : 5e-6) * cd.bn / 128;
-        c.step_s[0] = c.step_s[1] = c.step_s[2] = (long long)w.max_q * G <= 128 ? tile * 0.7 : tile;
+        c.step_s[0] = (long long)w.max_q * G <= 128 ? tile * 0.7 : tile;
         c.ramp_s = 10e-6;
         c.join_s = 3e-6;
         c.join_piece_s = 0.1e-6;
@@ -608,7 +623,8 @@ int pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cu
     a.chunk = p.chunk;
     a.ws_o = (float*)workspace;
     a.ws_ml = a.ws_o + (size_t)p.n_splits * batch->n_tok * n_heads * D;
-    const dim3 merge_grid((unsigned)(((size_t)batch->n_tok * n_heads + MERGE_WARPS - 1) / MERGE_WARPS));
+    const size_t out_rows = (size_t)batch->n_tok * n_heads;
+    const dim3 merge_grid((unsigned)(p.few ? out_rows : (out_rows + MERGE_WARPS - 1) / MERGE_WARPS));
     return dispatch(pages->kv_type, D, row_type, [&](auto kv, auto d, auto rows) {
         static std::atomic<uint64_t> few_set{0}, many_set{0};
         if (p.few) {

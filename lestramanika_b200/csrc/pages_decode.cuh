@@ -43,10 +43,11 @@ struct DecodeTile {
     static constexpr int CH = ROWB / 16;              // 16-byte chunks of a row
     static constexpr int KCH = CH / 4;                // chunks of a K row that a lane takes
     static constexpr int CELLB = cell_bytes(KV, D);
-    // 8-bit: 16 warps an SM in two CTAs with 12 KB of ring each (203 KB in all). BF16 cells are twice as large
-    // and cheaper to use: 12 warps in three CTAs with 16 KB each.
-    static constexpr int WARPS = KV == BF16 ? 4 : 8;
-    static constexpr int CTAS = KV == BF16 ? 3 : 2;
+    // 8-bit: 16 warps an SM with 12 KB of ring each (203 KB in all), in four CTAs: in two of eight warps, what a CTA does
+    // before its first and after its last cell is hidden less (16 sequences of 32768, 8 heads: 232 us instead of 199; 64
+    // ragged ones up to 4096: 89 instead of 81). BF16 cells are twice as large and cheaper to use: 12 warps with 16 KB.
+    static constexpr int WARPS = 4;
+    static constexpr int CTAS = KV == BF16 ? 3 : 4;
     static constexpr int STAGES = (KV == BF16 ? 2 : 3) * 128 / D;
     static constexpr int OPAD = D + 4;                // floats between output columns of a warp's partial
     static constexpr int RING = WARPS * STAGES * CELLB;
@@ -573,57 +574,61 @@ pages_decode_kernel(const AttnArgs a) {
     }
 }
 
-// Output row (t, h) from its pieces, one warp a row:
+// Output row (t, h) from its pieces:
 //   M = max m_i,  o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.
 // The number of pieces follows from the sequence as in the split kernel, so
-// pieces that never ran are never read.
+// pieces that never ran are never read. A row has one warp where there are many rows, and
+// all MERGE_WARPS, each with every fourth piece, behind the kernel for few rows: a decode of
+// one sequence has 32 rows of 16 pieces, and their loads are then all in flight.
 constexpr int MERGE_WARPS = 4;
 
 // ROWS_CTA: rows of the split kernel's blocks (0: it takes a sequence's rows together).
 template <int D, int ROWS, int STEP, int ROWS_CTA>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) pages_merge_kernel(const AttnArgs a) {
-    constexpr int E = D / 32;
+    constexpr int E = D / 32, RW = ROWS_CTA > 0 ? 1 : MERGE_WARPS;           // warps of a row
     const View& w = a.w;
-    const int lane = threadIdx.x & 31;
-    const size_t rows = (size_t)w.n_tok * a.H, row = (size_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = RW == 1 ? 0 : warp;
+    const size_t rows = (size_t)w.n_tok * a.H, row = RW == 1 ? (size_t)blockIdx.x * MERGE_WARPS + warp : blockIdx.x;
+    // The batch is read before the wait: the split kernel, all of whose CTAs run by now, has waited for its writers.
+    int tok = 0, head = 0, pieces = 0;
+    if (row < rows) {
+        tok = (int)(row / a.H);
+        head = (int)(row % a.H);
+        const int b = seq_of_row(w, tok, lane);
+        int row0, n, kv;
+        if (b < w.n_seqs && seq_bounds(w, b, row0, n, kv)) {
+            if constexpr (ROWS_CTA > 0) {
+                pieces = chunk_work<STEP, ROWS_CTA>(a, row0, n, kv, ((tok - row0) * a.G + head % a.G) / ROWS_CTA).pieces;
+            } else {
+                pieces = (span_of<STEP>(max(0, kv - n), kv - 1, a.window, a.sinks).n + a.chunk - 1) / a.chunk;
+            }
+        }
+    }
     griddep_wait();
     griddep_launch_dependents();
-    if (row >= rows) return;
-    const int tok = (int)(row / a.H), head = (int)(row % a.H);
-    const int b = seq_of_row(w, tok, lane);
-    if (b >= w.n_seqs) return;
-    int row0, n, kv;
-    if (!seq_bounds(w, b, row0, n, kv)) return;
-    int pieces;
-    if constexpr (ROWS_CTA > 0) {
-        pieces = chunk_work<STEP, ROWS_CTA>(a, row0, n, kv, ((tok - row0) * a.G + head % a.G) / ROWS_CTA).pieces;
-    } else {
-        pieces = (span_of<STEP>(max(0, kv - n), kv - 1, a.window, a.sinks).n + a.chunk - 1) / a.chunk;
-    }
     if (pieces <= 1) return;
-    // lane i holds piece i's statistics (pieces beyond 32: the loop below takes 32 at a time)
     float M = -INFINITY;
     for (int i = lane; i < pieces; i += 32) M = fmaxf(M, a.ws_ml[2 * (i * rows + row)]);
     #pragma unroll
     for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
     const float Mz = M == -INFINITY ? 0.f : M;
-    float L = 0.f, y[E];
-    #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = 0.f;
-    for (int i0 = 0; i0 < pieces; i0 += 32) {
+    float L = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    // 32 of the warp's pieces a time: a lane holds the statistics of one.
+    for (int i0 = part; i0 < pieces; i0 += 32 * RW) {
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (i0 + lane < pieces) ml = *reinterpret_cast<const float2*>(a.ws_ml + 2 * ((size_t)(i0 + lane) * rows + row));
+        const int own = i0 + lane * RW;
+        if (own < pieces) ml = *reinterpret_cast<const float2*>(a.ws_ml + 2 * ((size_t)own * rows + row));
         const float f = ex2(ml.x - Mz);
         L += f * ml.y;
-        const int m = min(32, pieces - i0);
+        const int m = min(32, (pieces - i0 + RW - 1) / RW);
         #pragma unroll 4
         for (int i = 0; i < m; ++i) {
             const float fi = __shfl_sync(0xffffffffu, f, i);
-            const float* src = a.ws_o + ((size_t)(i0 + i) * rows + row) * D + E * lane;
+            const float* src = a.ws_o + ((size_t)(i0 + i * RW) * rows + row) * D + E * lane;
             if (E == 4) {
                 const float4 v = *reinterpret_cast<const float4*>(src);
                 y[0] = fmaf(fi, v.x, y[0]); y[1] = fmaf(fi, v.y, y[1]);
-                y[E - 2] = fmaf(fi, v.z, y[E - 2]); y[E - 1] = fmaf(fi, v.w, y[E - 1]);
+                y[2] = fmaf(fi, v.z, y[2]); y[3] = fmaf(fi, v.w, y[3]);
             } else {
                 const float2 v = *reinterpret_cast<const float2*>(src);
                 y[0] = fmaf(fi, v.x, y[0]); y[1] = fmaf(fi, v.y, y[1]);
@@ -632,15 +637,29 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) pages_merge_kernel(const Att
     }
     #pragma unroll
     for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+    if constexpr (RW > 1) {
+        __shared__ float4 s_y[RW][32];
+        __shared__ float s_l[RW];
+        s_y[warp][lane] = make_float4(y[0], y[1], y[2], y[3]);
+        if (lane == 0) s_l[warp] = L;
+        __syncthreads();
+        if (warp) return;
+        #pragma unroll
+        for (int k = 1; k < RW; ++k) {
+            const float4 v = s_y[k][lane];
+            y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
+            L += s_l[k];
+        }
+    }
     const float inv = 1.0f / (L == 0.f ? 1.0f : L);
     const size_t at = (size_t)tok * a.out_stride + (size_t)head * D + E * lane;
     if (ROWS == PICKLE_CUDA_ROW_F32) {
         float* dst = reinterpret_cast<float*>(a.out) + at;
-        if (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0] * inv, y[1] * inv, y[E - 2] * inv, y[E - 1] * inv);
+        if (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
         else *reinterpret_cast<float2*>(dst) = make_float2(y[0] * inv, y[1] * inv);
     } else {
         __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.out) + at;
-        if (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(bf16x2(y[0] * inv, y[1] * inv), bf16x2(y[E - 2] * inv, y[E - 1] * inv));
+        if (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(bf16x2(y[0] * inv, y[1] * inv), bf16x2(y[2] * inv, y[3] * inv));
         else *reinterpret_cast<uint32_t*>(dst) = bf16x2(y[0] * inv, y[1] * inv);
     }
 }

@@ -73,7 +73,8 @@ PCU_DEV Place place_of(const View& w, int t, int rope_len, int lane) {
     Place x{NOT_OURS, 0, 0, 0u};
     const int b = t < w.n_tok ? seq_of_row(w, t, lane) : w.n_seqs;
     int row0, n, kv;
-    if (b >= w.n_seqs || !seq_bounds(w, b, row0, n, kv)) return x;
+    // (t - row0 lies outside [0, n) only where q_start does not ascend.)
+    if (b >= w.n_seqs || !seq_bounds(w, b, row0, n, kv) || t < row0 || t - row0 >= n) return x;
     x.pos = kv - n + (t - row0);
     x.state = NO_PLACE;
     if (x.pos < 0) return x;

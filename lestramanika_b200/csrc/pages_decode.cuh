@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) pages_merge_kernel(const Att
         head = (int)(row % a.H);
         const int b = seq_of_row(w, tok, lane);
         int row0, n, kv;
-        if (b < w.n_seqs && seq_bounds(w, b, row0, n, kv)) {
+        if (b < w.n_seqs && seq_bounds(w, b, row0, n, kv) && tok >= row0 && tok - row0 < n) {
             if constexpr (ROWS_CTA > 0) {
                 pieces = chunk_work<STEP, ROWS_CTA>(a, row0, n, kv, ((tok - row0) * a.G + head % a.G) / ROWS_CTA).pieces;
             } else {

@@ -217,6 +217,8 @@ class KVPages:
                 raise PickleError(ERR_ARG, "KVPages", "q, k and v have one element type")
         if vt != rt:
             raise PickleError(ERR_ARG, "KVPages", "q, k and v have one element type")
+        if batch.n_tok == 0:                 # tensors without rows have no address
+            return
         self._run(self._lib.pickle_cuda_pages_append_dev, "pickle_cuda_pages_append_dev", self._refs[layer],
                   batch._ref, H, rt, qp or None, qs, kp, ks, vp, vs, *self._rope_args, self.half, self.rope_len, ot,
                   op or None, os_, st)
@@ -228,6 +230,8 @@ class KVPages:
         vp, vt, vs = self._rows(v_out, self.HK, batch.n_tok, "v_out")
         if rt != vt:
             raise PickleError(ERR_ARG, "KVPages", "k_out and v_out have one element type")
+        if batch.n_tok == 0:
+            return
         self._run(self._lib.pickle_cuda_pages_read_dev, "pickle_cuda_pages_read_dev", self._refs[layer], batch._ref,
                   rt, kp, ks, vp, vs, st)
 
@@ -244,12 +248,16 @@ class KVPages:
             raise PickleError(ERR_ARG, "KVPages", "q and out have one element type")
         if window < 0 or sinks < 0:
             raise PickleError(ERR_ARG, "KVPages", "window and sinks are not negative")
+        if batch.n_tok == 0:
+            return
         key = (self, H, rt, window, sinks)
         need = batch._ws.get(key)
         if need is None:
             need = batch._ws[key] = self.attn_workspace(batch, H, rt, window, sinks)
         wp = 0
         if workspace is not None:
+            if not workspace.is_contiguous() or workspace.get_device() != self.device:
+                raise PickleError(ERR_ARG, "KVPages", f"workspace is contiguous and on {self._dev}")
             wp, need = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         elif need:
             workspace = self._scratch(need, stream)

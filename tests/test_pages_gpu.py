@@ -494,3 +494,58 @@ def test_ragged_decodes(rows, lens):
     first = _check_attn(B, 3, rows, q=q)
     assert torch.equal(first, _check_attn(B, 3, rows, q=q))             # the same bits again
     _check_attn(B, 3, rows, 300, 20, q=q)
+
+
+def test_starts_that_do_not_ascend_touch_nothing_else():
+    """q_start [0, 5, 3, 4]: the second sequence has -2 rows, row 4 lies in no sequence, and row 3 is the third's. What has
+    rows is written and attended to, and the error word says the rest."""
+    B = R.Batch("i8", 2, 128, 16, [40, 32, 48], [5, 0, 1], 51)
+    cache, H = _cache(B), 6
+    kv, table, _ = B.tensors()
+    start = torch.tensor([0, 5, 3, 4], dtype=torch.int32, device=DEV)
+    batch = PageBatch(kv, table, q_start=start, n_tok=6, max_q=5, max_kv=48)
+    q = torch.randn((6, H, 128), generator=torch.Generator().manual_seed(1)).to(DEV)
+    out = torch.full_like(q, 7.0)
+    for window in (0, 20):
+        cache.attn_dev(0, batch, q, out, window=window)
+        with pytest.raises(PickleError):
+            cache.sync()
+    pool = B.pool.clone()
+    k = torch.randn((6, 2, 128), generator=torch.Generator().manual_seed(2)).to(DEV)
+    cache.append_dev(0, batch, k, k)
+    with pytest.raises(PickleError):
+        cache.sync()
+    k_out, v_out = torch.full_like(k, 7.0), torch.full_like(k, 7.0)
+    cache.read_dev(0, batch, k_out, v_out)
+    with pytest.raises(PickleError):
+        cache.sync()
+    assert torch.equal(out[5], torch.full_like(out[5], 7.0)) and torch.equal(k_out[4:], torch.full_like(k_out[4:], 7.0))
+    changed = (pool != B.pool).view(B.n_pages, -1).any(1).nonzero().flatten().tolist()
+    assert set(changed) <= {p for row in B.tensors()[1].tolist() for p in row if p >= 0}
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+def test_calls_without_rows(rows):
+    B = R.Batch("i8", 2, 64, 16, [20, 0], [0, 0], 52)
+    cache = _cache(B)
+    kv, table, start = B.tensors()
+    batch = PageBatch(kv, table, q_start=start)
+    before = B.pool.clone()
+    k, q = (torch.empty((0, h, 64), dtype=R.ROWS[rows], device=DEV) for h in (2, 4))
+    cache.append_dev(0, batch, k, k, q=q, q_out=q)
+    cache.read_dev(0, batch, k, k)
+    cache.attn_dev(0, batch, q, q)
+    cache.sync()
+    assert torch.equal(before, B.pool)
+
+
+def test_refused_workspaces():
+    B = R.Batch("i8", 1, 128, 16, [4000], [1], 53)
+    cache, batch = _cache(B), _batch(B)
+    q = B.randn(1, 4, 128)
+    need = cache.attn_workspace(batch, 4, 0)
+    assert need > 0
+    for ws in (torch.empty(need - 1, dtype=torch.uint8, device=DEV), torch.empty(need, dtype=torch.uint8),
+               torch.empty(2 * need, dtype=torch.uint8, device=DEV)[::2], torch.empty(need + 8, dtype=torch.uint8, device=DEV)[8:]):
+        with pytest.raises(PickleError):
+            cache.attn_dev(0, batch, q, torch.empty_like(q), workspace=ws)

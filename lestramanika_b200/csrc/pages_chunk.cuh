@@ -200,6 +200,24 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     const int n_all = twin ? n_tiles : max(n_a, n_b);
     auto tile_of = [&](int x, int i) { return twin ? 2 * i + x : i; };      // tile x's i-th tile of keys
 
+    // Softmax warps: 16 of their tile's q rows each, D / 8 lanes a row. The first QA of the QSTEPS loads are on their
+    // way while barriers and TMEM are set up (asked for after that, four by four, q was there 3 us later).
+    constexpr int LPR = D / 8, QSTEPS = 16 * LPR / 32, QA = ROWS == PICKLE_CUDA_ROW_F32 && QSTEPS > 4 ? 4 : QSTEPS;
+    const int qx = warp >> 3;                                      // their tile of rows
+    const bool takes_q = warp < CHUNK_STAGE_WARP && (qx ? has_b && n_b > 0 : n_a > 0);
+    const int q_row = (warp & 7) * 16 + lane / LPR;                // first of the lane's rows
+    RawRow8<ROWS> q_raw[QA];
+    auto ask_q = [&](int s0) {
+        #pragma unroll
+        for (int k = 0; k < QA; ++k) {
+            const int q = cw.r0 + qx * 128 + q_row + (s0 + k) * (32 / LPR), t = div_group(q, a);
+            q_raw[k].clear();
+            if (q < cw.R)
+                q_raw[k].load(a.q, (size_t)(cw.row0 + t) * a.q_stride + (size_t)(hk * a.G + q - t * a.G) * D + 8 * (lane % LPR));
+        }
+    };
+    if (takes_q) ask_q(0);
+
     const uint32_t base_u32 = smem_u32(base);
     if (base_u32 & 1023u) {                        // the operands' swizzle goes by address bits
         record_error(w.err, PCU_DEVERR_ARG);
@@ -542,34 +560,26 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         const int tok = div_group(r, a), head = hk * a.G + r - tok * a.G;
         const int p = live ? cw.pos0 + tok : -1;
         bool ok = true;
-        if (n_x > 0 && x == xr) {
-            // 16 of the tile's q rows a warp into shared memory, in the operand order: D / 8 lanes a row.
-            constexpr int LPR = D / 8, RPS = 32 / LPR, STEPS = 16 / RPS;
-            const int i0 = 8 * (lane % LPR), tr0 = (warp & 7) * 16;
-            #pragma unroll 1
-            for (int s0 = 0; s0 < STEPS; s0 += 4) {
-                Row8 v[4];
+        if (takes_q) {
+            // q into shared memory, in the operand order.
+            const int i0 = 8 * (lane % LPR);
+            #pragma unroll
+            for (int s0 = 0; s0 < QSTEPS; s0 += QA) {
+                if (s0) ask_q(s0);
                 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int q = cw.r0 + x * 128 + tr0 + (s0 + k) * RPS + lane / LPR, t = div_group(q, a);
-                    v[k].a = v[k].b = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (q < cw.R)
-                        v[k] = load_row8<ROWS>(a.q, (size_t)(cw.row0 + t) * a.q_stride + (size_t)(hk * a.G + q - t * a.G) * D + i0);
-                }
-                #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int r_t = tr0 + (s0 + k) * RPS + lane / LPR;            // row of the tile
+                for (int k = 0; k < QA; ++k) {
+                    const int r_t = q_row + (s0 + k) * (32 / LPR);                // row of the tile
+                    const Row8 v = q_raw[k].row();
                     float qs = 1.f;
                     if (!BF) {
-                        uint32_t m = max(amax_bits(v[k].a), amax_bits(v[k].b));
+                        uint32_t m = max(amax_bits(v.a), amax_bits(v.b));
                         #pragma unroll
                         for (int y = 1; y < LPR; y <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, y));
                         const uint32_t e = min(268u - (m >> 23), 254u);
                         qs = __uint_as_float(e << 23);
                         if (lane % LPR == 0) aux.qexp[x * 128 + r_t] = (unsigned char)e;
                     }
-                    const float e[8] = {v[k].a.x * qs, v[k].a.y * qs, v[k].a.z * qs, v[k].a.w * qs,
-                                        v[k].b.x * qs, v[k].b.y * qs, v[k].b.z * qs, v[k].b.w * qs};
+                    const float e[8] = {v.a.x * qs, v.a.y * qs, v.a.z * qs, v.a.w * qs, v.b.x * qs, v.b.y * qs, v.b.z * qs, v.b.w * qs};
                     constexpr int o1 = KV == I8 ? 2 : 1, o2 = KV == I8 ? 1 : 2;
                     uint32_t q0[NP], q1[NP], q2[NP], q3[NP];
                     split_parts<BF, NP>(e[0], e[o1], q0);

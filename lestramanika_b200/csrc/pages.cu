@@ -355,7 +355,7 @@ int allow_smem(void (*fn)(Args...), int bytes, std::atomic<uint64_t>& done) {
 struct Plan {
     bool few;           // the kernel for few rows
     int blocks;         // else: blocks of rows a sequence may have
-    int n_splits, chunk;
+    int n_splits, chunk, chunk_min, target;
 };
 
 // How many pieces the keys of `groups` independent streams of `steps` steps
@@ -365,7 +365,7 @@ struct Plan {
 // join (a launch, and a piece at a time) and its traffic. The host knows the longest
 // stream only: where streams may differ, what counts is this time plus that
 // of lengths spread evenly from none to `steps`, the work shared out with
-// half a piece's time left over (32 sequences of 8192 keys, 8 heads: one piece 130 us, 8 pieces 72 where they are
+// half a piece's time left over (32 sequences of 8192 keys, 8 heads: one piece 130 us, 8 pieces 71 where they are
 // ragged, up to 6% lost where they are not).
 struct Costs {
     int per_sm;
@@ -461,7 +461,7 @@ Plan plan_attn(const View& w, int kv_type, int D, int row_type, int H, int windo
         c.join_piece_s = 0.1e-6;
     } else {
         c.per_sm = 1;
-        c.ragged = false;
+        c.ragged = false;            // see piece_steps
         // A tile of 128 keys takes this long with 256 rows, and two thirds of it with 128 or fewer.
         const double tile = (row_type != PICKLE_CUDA_ROW_F32 ? 2.5e-6 : D == 64 ? 3.1e-6 : kv_type == BF16 ? 8e-6 : 5e-6) * cd.bn / 128;
         c.step_s[0] = (long long)w.max_q * G <= 128 ? tile * 0.7 : tile;
@@ -470,10 +470,19 @@ Plan plan_attn(const View& w, int kv_type, int D, int row_type, int H, int windo
         c.join_piece_s = 0.1e-6;
     }
     p.n_splits = plan_pieces(groups, steps, sms, c);
-    // Knob for sweeps of the piece count.
-    if (const char* env = getenv("PICKLE_CUDA_PAGES_SPLITS"))
-        if (atoi(env) > 0) p.n_splits = atoi(env) < steps ? atoi(env) : (int)steps;
-    p.chunk = (int)((steps + p.n_splits - 1) / p.n_splits);
+    // Knob for sweeps of the piece count: that many, as if all sequences were the longest.
+    const char* env = getenv("PICKLE_CUDA_PAGES_SPLITS");
+    const int asked = env ? atoi(env) : 0;
+    if (asked > 0) p.n_splits = asked < steps ? asked : (int)steps;
+    p.chunk = p.chunk_min = (int)((steps + p.n_splits - 1) / p.n_splits);
+    p.target = 0;
+    // Sequences may be shorter: room for twice the pieces of each, no more in all. Not with a window, under which long ones
+    // are alike, nor with several blocks of rows, which end at different keys.
+    if (!p.few && asked <= 0 && p.n_splits > 1 && window == 0 && p.blocks == 1 && w.n_seqs <= TARGET_SEQS) {
+        p.target = w.n_seqs * p.n_splits;
+        p.n_splits = 2 * p.n_splits < steps ? 2 * p.n_splits : (int)steps;
+        p.chunk_min = (int)((steps + p.n_splits - 1) / p.n_splits);
+    }
     return p;
 }
 
@@ -622,6 +631,8 @@ int pickle_cuda_pages_attn_dev(const pickle_cuda_pages_t* pages, const pickle_cu
     if (need && (!workspace || (uintptr_t)workspace % 16 || ws_bytes < need)) return PICKLE_ERR_ARG;
     a.n_splits = p.n_splits;
     a.chunk = p.chunk;
+    a.chunk_min = p.chunk_min;
+    a.target = p.target;
     a.ws_o = (float*)workspace;
     a.ws_ml = a.ws_o + (size_t)p.n_splits * batch->n_tok * n_heads * D;
     const size_t out_rows = (size_t)batch->n_tok * n_heads;

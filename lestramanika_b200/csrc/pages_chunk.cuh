@@ -183,11 +183,12 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     const int b = blockIdx.x / w.HK, hk = blockIdx.x % w.HK;
     const int qb = gridDim.y - 1 - blockIdx.y, split = blockIdx.z;       // later rows (more keys) first
     int row0, n, kv;
+    const int chunk = piece_steps<BN>(a, lane);
     if (!seq_bounds(w, b, row0, n, kv)) return;
     if (qb * T::ROWS_CTA >= n * a.G) return;
-    const ChunkWork cw = chunk_work<BN, T::ROWS_CTA>(a, row0, n, kv, qb);
+    const ChunkWork cw = chunk_work<BN, T::ROWS_CTA>(a, row0, n, kv, qb, chunk);
     if (split > 0 && split >= cw.pieces) return;
-    const int t0 = split * a.chunk, t1 = min(cw.span.n, t0 + a.chunk), n_tiles = t1 - t0;
+    const int t0 = split * chunk, t1 = min(cw.span.n, t0 + chunk), n_tiles = t1 - t0;
     // Tile A ends with an earlier position than the block: the key tiles it has to see.
     const bool has_b = T::TILES == 2 && cw.r0 + 128 < cw.R;
     // Rows for one tile only: both work on it, A on the even tiles of keys and B on the odd ones, so that one's softmax

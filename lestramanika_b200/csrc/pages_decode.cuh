@@ -220,12 +220,13 @@ pages_decode_kernel(const AttnArgs a) {
     griddep_launch_dependents();
     const int b = blockIdx.x / w.HK, hk = blockIdx.x % w.HK, split = blockIdx.y;
     int row0, n, kv;
+    const int chunk = a.chunk;
     if (!seq_bounds(w, b, row0, n, kv) || n == 0) return;
     const int G = a.G, R = n * G, pos0 = kv - n;       // rows of this KV head; position of the first token
     const Span span = span_of<CELL>(max(0, pos0), kv - 1, a.window, a.sinks);
-    const int pieces = (span.n + a.chunk - 1) / a.chunk;
+    const int pieces = (span.n + chunk - 1) / chunk;
     if (split > 0 && split >= pieces) return;
-    const int e0 = split * a.chunk, e1 = min(span.n, e0 + a.chunk);
+    const int e0 = split * chunk, e1 = min(span.n, e0 + chunk);
     const int mine = (e1 - e0 - warp + W - 1) / W;     // cells e0 + warp, e0 + warp + W, ... of the span
 
     // What the warp has to know of 32 of its cells, one a lane: where the cell lies in the pool and which of
@@ -591,6 +592,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) pages_merge_kernel(const Att
     const size_t rows = (size_t)w.n_tok * a.H, row = RW == 1 ? (size_t)blockIdx.x * MERGE_WARPS + warp : blockIdx.x;
     // The batch is read before the wait: the split kernel, all of whose CTAs run by now, has waited for its writers.
     int tok = 0, head = 0, pieces = 0;
+    const int chunk = ROWS_CTA > 0 ? piece_steps<STEP>(a, lane) : a.chunk;
     if (row < rows) {
         tok = (int)(row / a.H);
         head = (int)(row % a.H);
@@ -598,9 +600,9 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) pages_merge_kernel(const Att
         int row0, n, kv;
         if (b < w.n_seqs && seq_bounds(w, b, row0, n, kv) && tok >= row0 && tok - row0 < n) {
             if constexpr (ROWS_CTA > 0) {
-                pieces = chunk_work<STEP, ROWS_CTA>(a, row0, n, kv, ((tok - row0) * a.G + head % a.G) / ROWS_CTA).pieces;
+                pieces = chunk_work<STEP, ROWS_CTA>(a, row0, n, kv, ((tok - row0) * a.G + head % a.G) / ROWS_CTA, chunk).pieces;
             } else {
-                pieces = (span_of<STEP>(max(0, kv - n), kv - 1, a.window, a.sinks).n + a.chunk - 1) / a.chunk;
+                pieces = (span_of<STEP>(max(0, kv - n), kv - 1, a.window, a.sinks).n + chunk - 1) / chunk;
             }
         }
     }

@@ -549,3 +549,20 @@ def test_refused_workspaces():
                torch.empty(2 * need, dtype=torch.uint8, device=DEV)[::2], torch.empty(need + 8, dtype=torch.uint8, device=DEV)[8:]):
         with pytest.raises(PickleError):
             cache.attn_dev(0, batch, q, torch.empty_like(q), workspace=ws)
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,most", [([4000, 30, 1, 700, 0, 2000], 4000), ([600, 590], 16000), ([3000], 3000),
+                                       ([2500] + [17] * 60, 2500), ([500] * 128, 2000), ([500] * 129, 2000)])
+def test_chunks_of_ragged_contexts(rows, lens, most):
+    """Pieces are cut to what the sequences' lengths say, not to the longest that the host allows for."""
+    new = [min(9, m) for m in lens]
+    B = R.Batch("i8", 1, 128, 32, lens, new, 61)
+    kv, table, start = B.tensors()
+    wide = torch.full((len(lens), -(-most // 32)), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    batch = PageBatch(kv, wide, q_start=start, n_tok=B.n_tok, max_q=9, max_kv=most)
+    q = B.randn(B.n_tok, 4, 128).to(R.ROWS[rows])
+    first = _check_attn(B, 4, rows, q=q, batch=batch)
+    assert torch.equal(first, _check_attn(B, 4, rows, q=q, batch=batch))
+    _check_attn(B, 4, rows, 300, 20, q=q, batch=batch)

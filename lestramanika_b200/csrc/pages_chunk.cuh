@@ -90,6 +90,10 @@ PCU_DEV void bulk_g2s_at(uint32_t dst, const void* src, uint32_t bytes, uint64_t
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+// Bytes that a phase of the barrier waits for, besides its arrivals.
+PCU_DEV void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 PCU_DEV void sts128(uint32_t to, const uint4& v) {
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -219,13 +223,61 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     };
     if (takes_q) ask_q(0);
 
+    // Loading warps: lane c < NCT looks after cell c of a tile. need: its keys that some row sees; a page id is asked for two
+    // tiles before it is used, and the cell's bytes are asked for in L2 a tile before they are copied.
+    const uint32_t cpp = w.page_size / CELL;
+    struct Cell {
+        uint32_t at, need;
+    };
+    auto ask = [&](int j, int& id) {
+        Cell x{0u, 0u};
+        id = 0;
+        if (j < n_all && lane < NCT) {
+            const int k0 = cw.span.step(t0 + j) * BN + lane * CELL;
+            x.need = bits_below(cw.last + 1 - k0) & 0xffffu;
+            if (k0 < cw.span.lo_key) x.need &= ~bits_below(cw.span.lo_key - k0) | bits_below(a.sinks - k0);
+            if (x.need) {
+                const uint32_t cell = (uint32_t)k0 / CELL, page = cell / cpp;
+                id = w.table[(size_t)b * w.table_stride + page];
+                x.at = cell - page * cpp;
+            }
+        }
+        return x;
+    };
+    // With its page's id: the cell in the pool; on a bad page none of its keys is there.
+    auto look = [&](Cell x, int id) {
+        if (x.need) {
+            if ((unsigned)id < (unsigned)w.n_pages) {
+                x.at += ((uint32_t)id * w.HK + hk) * cpp;
+            } else {
+                x.need = 0x10000u;
+                record_error(w.err, PCU_DEVERR_ARG);
+            }
+        }
+        return x;
+    };
+    auto want = [](const Cell& x) { return (x.need & 0xffffu) != 0; };
+    auto cell_at = [&](const Cell& x) { return w.pool + (size_t)x.at * cell_bytes(KV, D); };
+    // The first tiles' pages are looked up, and the first tile asked for in L2, while the rest is set up.
+    Cell x0{0u, 0u}, x1{0u, 0u}, far{0u, 0u};
+    int id2 = 0;
+    if (warp >= CHUNK_LOAD_WARP && warp <= CHUNK_LOAD_WARP + 1) {
+        int id0, id1;
+        x0 = ask(0, id0);
+        x1 = ask(1, id1);
+        far = ask(2, id2);
+        x0 = look(x0, id0);
+        x1 = look(x1, id1);
+        if (warp > CHUNK_LOAD_WARP && want(x0)) bulk_prefetch_l2(cell_at(x0), cell_bytes(KV, D));
+    }
+
     const uint32_t base_u32 = smem_u32(base);
     if (base_u32 & 1023u) {                        // the operands' swizzle goes by address bits
         record_error(w.err, PCU_DEVERR_ARG);
         return;
     }
     uint64_t* bars = aux.bars;
-    if (tid == 0) {
+    if (tid == CHUNK_THREADS - 32) {               // of a warp that has nothing else to do here
         for (int x = 0; x < 2; ++x) {
             mbar_init(&bars[Q_FULL + x], 8);
             mbar_init(&bars[S_FULL + x], 2);      // the products, and the thread that saw the tile's words
@@ -320,45 +372,6 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         } else if (warp <= CHUNK_LOAD_WARP + 1) {
             const int v = warp - CHUNK_LOAD_WARP;          // K or V: a copy costs its issuer some 80 cycles
             // ---------------- pages -> shared memory ----------------
-            // Lane c < NCT looks after cell c of a tile. need: its keys that some row sees; a page id is asked for two
-            // tiles before it is used, and the cell's bytes are asked for in L2 a tile before they are copied.
-            const uint32_t cpp = w.page_size / CELL;
-            struct Cell {
-                uint32_t at, need;
-            };
-            auto ask = [&](int j, int& id) {
-                Cell x{0u, 0u};
-                id = 0;
-                if (j < n_all && lane < NCT) {
-                    const int k0 = cw.span.step(t0 + j) * BN + lane * CELL;
-                    x.need = bits_below(cw.last + 1 - k0) & 0xffffu;
-                    if (k0 < cw.span.lo_key) x.need &= ~bits_below(cw.span.lo_key - k0) | bits_below(a.sinks - k0);
-                    if (x.need) {
-                        const uint32_t cell = (uint32_t)k0 / CELL, page = cell / cpp;
-                        id = w.table[(size_t)b * w.table_stride + page];
-                        x.at = cell - page * cpp;
-                    }
-                }
-                return x;
-            };
-            // With its page's id: the cell in the pool; on a bad page none of its keys is there.
-            auto look = [&](Cell x, int id) {
-                if (x.need) {
-                    if ((unsigned)id < (unsigned)w.n_pages) {
-                        x.at += ((uint32_t)id * w.HK + hk) * cpp;
-                    } else {
-                        x.need = 0x10000u;
-                        record_error(w.err, PCU_DEVERR_ARG);
-                    }
-                }
-                return x;
-            };
-            auto want = [](const Cell& x) { return (x.need & 0xffffu) != 0; };
-            auto cell_at = [&](const Cell& x) { return w.pool + (size_t)x.at * cell_bytes(KV, D); };
-            int id0, id1, id2;
-            Cell x0 = ask(0, id0), x1 = ask(1, id1), far = ask(2, id2);
-            x0 = look(x0, id0);
-            x1 = look(x1, id1);
             bool ok = true;
             auto wait = [&](int bar, int phase) { ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars[bar], phase & 1) && !aborted()); };
             // 8-bit: scale words of keys 32 q + lane of the next tile; V's reference exponents.
@@ -390,6 +403,28 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                 if (v && want(x1)) bulk_prefetch_l2(cell_at(x1), cell_bytes(KV, D));
                 const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, want(x0))) * CELL * D * elem_bytes(KV);
                 const int bad = __any_sync(0xffffffffu, x0.need >> 16);
+                if (j >= STAGES) wait((v ? V_EMPTY : K_EMPTY) + st, j / STAGES - 1);
+                if (!ok) break;
+                const uint32_t dst = base_u32 + T::SMEM_KV + st * T::STAGE + v * T::KV_TILE + (BF ? lane * CELL * 128 : T::raw_at(lane * CELL));
+                uint64_t* bar = &bars[(v ? RAW_V : BF ? K_FULL : RAW_K) + st];
+                // BF16: two boxes of 64 columns and 16 rows for each of a cell's K and V. 8-bit: a cell's codes, where
+                // staging turns them over; they are asked for before the scales, which come from the same cells, are looked at.
+                auto copy = [&]() {
+                    __syncwarp();
+                    if (want(x0)) {
+                        if constexpr (BF) {
+                            for (int h = 0; h < D / 64; ++h)
+                                tma_load_2d(dst + h * T::KV_HALF, &tm, 64 * h, (int)(x0.at * 2 * CELL + v * CELL), bar);
+                        } else {
+                            bulk_g2s_at(dst, cell_at(x0) + (v ? v_row(KV, D, 0) : 0), CELL * D, bar);
+                        }
+                    }
+                    ++issued;
+                };
+                if (!BF) {
+                    if (lane == 0 && bytes) mbar_expect_tx(bar, bytes);
+                    copy();
+                }
                 uint32_t km[BN / 32], vm = 0;
                 if (!BF && v == 0) {
                     // K: one reference for 32 keys. V: a reference moves where the tile's largest exponent passes it by
@@ -412,8 +447,6 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                     }
                     ev = vm;
                 }
-                if (j >= STAGES) wait((v ? V_EMPTY : K_EMPTY) + st, j / STAGES - 1);
-                if (!ok) break;
                 if (lane < NCT) s_need[v][i][lane] = x0.need;
                 if (!BF) {
                     #pragma unroll
@@ -427,23 +460,14 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                         for (int k = 0; k < 4; ++k) s_km[i][k] = km[k * (BN / 32) / 4];
                     }
                 }
-                // BF16: two boxes of 64 columns and 16 rows for each of a cell's K and V. 8-bit: a cell's codes, where
-                // staging turns them over.
-                const uint32_t dst = base_u32 + T::SMEM_KV + st * T::STAGE + v * T::KV_TILE + (BF ? lane * CELL * 128 : T::raw_at(lane * CELL));
-                uint64_t* bar = &bars[(v ? RAW_V : BF ? K_FULL : RAW_K) + st];
                 __syncwarp();
-                if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
-                __syncwarp();
-                if (want(x0)) {
-                    if constexpr (BF) {
-                        for (int h = 0; h < D / 64; ++h)
-                            tma_load_2d(dst + h * T::KV_HALF, &tm, 64 * h, (int)(x0.at * 2 * CELL + v * CELL), bar);
-                    } else {
-                        bulk_g2s_at(dst, cell_at(x0) + (v ? v_row(KV, D, 0) : 0), CELL * D, bar);
-                    }
+                if (BF) {
+                    if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+                    copy();
+                } else {
+                    if (lane == 0) mbar_arrive(bar);
+                    scales(x1);
                 }
-                ++issued;
-                if (!BF) scales(x1);
                 x0 = x1;
                 x1 = look(far, id2);
                 far = ask(j + 3, id2);

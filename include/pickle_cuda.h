@@ -485,12 +485,17 @@ PICKLE_CUDA_API int  pickle_cuda_pages_read_dev(const pickle_cuda_pages_t* pages
  * positions included: out = softmax(q . k / sqrtf(D)) v over the keys at
  * positions j <= p of a query at position p and, when window > 0, only those
  * with j > p - window or j < sinks. kv_head = h * HK / H, H / HK from 1 to 8.
- * q, out [n_tok][n_heads][D] of row_type, accumulation in F32; F32 rows keep
- * F32 accuracy, BF16 rows round the softmax weights to BF16 where
- * max_q * H / HK > 8. Pages
- * that no row of the call can see are never touched (their table entries may
- * be stale). A row that sees no key gives zeros. Keys on a page outside
- * the pool are left out and recorded in the error word.
+ * q, out [n_tok][n_heads][D] of row_type (out may be q), accumulation in
+ * F32. F32 rows keep F32 accuracy. With BF16 rows the softmax weights are
+ * rounded to F16 (2^-12 of the weight) on 8-bit pages; on BF16 pages to BF16
+ * (2^-9) where max_q * H / HK > 8 and to two BF16 numbers where it is not.
+ * Pages that no row of the call can see are never touched (their table
+ * entries may be stale). A row that sees no key gives zeros. Keys on a page
+ * outside the pool are left out and recorded in the error word. A k or v
+ * element that is not finite makes the rows that see it NaN (of a v element
+ * the whole row or the elements next to it) and no other row.
+ * The answers depend on the batch's bounds in their last bits only, and are
+ * the same bits for the same call.
  * workspace: pickle_cuda_pages_workspace(...) device bytes, 16-byte aligned;
  * calls that may overlap on the GPU need one each. */
 PICKLE_CUDA_API size_t pickle_cuda_pages_workspace(const pickle_cuda_pages_t* pages, const pickle_cuda_batch_t* batch,

@@ -97,6 +97,10 @@ PCU_DEV bool sees(int p, int j, int window, int sinks) {
     return j <= p && (window <= 0 || j > p - window || j < sinks);
 }
 
+// Whether one of two BF16 numbers is not finite.
+PCU_DEV bool bf16x2_bad(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+PCU_DEV bool bf16x8_bad(const uint4& x) { return bf16x2_bad(x.x) || bf16x2_bad(x.y) || bf16x2_bad(x.z) || bf16x2_bad(x.w); }
+
 // The rows and keys of one block of ROWS_CTA rows (a row: a token and a query
 // head of its KV head's group), for the kernel that takes them in blocks.
 struct ChunkWork {

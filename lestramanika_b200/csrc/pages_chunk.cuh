@@ -10,8 +10,7 @@
 //               layout (128-byte swizzle), 8-bit pages with bulk copies of the
 //               codes into the place of their operands, and their scales;
 //   warps 16-19 turn a tile's codes in place into 16-bit operands (K-major K,
-//               MN-major V);
-//               of BF16 pages they only clear V rows that no row sees;
+//               MN-major V); of BF16 pages they only clear V rows that no row sees;
 //   warp 20     one lane issues tcgen05.mma: S_X = Q_X K^T, O_X += P_X V,
 //               P_X read from TMEM, in the order PV_A, S_A, PV_B, S_B so that one
 //               tile's softmax runs under the other's products;
@@ -33,6 +32,17 @@
 // F32 rows: q and P are sums of two F16 (22 bits) or three BF16 (24 bits)
 // numbers with a product each, which keeps F32 accuracy at two or three times
 // the products.
+//
+// What bounds it, by a tile of 128 keys and 256 rows: the products take 2048
+// tensor cycles a part of q and p at D = 128 (1.1 us at 1.9 GHz), the softmax of both tiles
+// the issue slots of about 2 us, under which the products run: 2.25 us with BF16 rows on BF16
+// pages, 2.6 on 8-bit ones, whose codes four warps turn over meanwhile; F32 rows 4.9 and 8.1 (two and three
+// operands, tiles of 64 keys). Twins, 128 rows or fewer: 1.5 and 2.0. An item of 256 rows adds about 10 us
+// that nothing hides, one CTA filling an SM: page ids and q (3 us), the first
+// keys and softmax (5 us), the epilogue (3 us).
+// Measured (us): 2048 tokens on 8192, 32 / 8 heads, E4M3: 377 (820 TFLOP/s); 4 prompts of 2048, 32 / 32 heads,
+// BF16: 228 (604); 2 ragged ones up to 4001, window 1000, F32, D = 64, int8: 113;
+// 8 x 16 tokens on ragged contexts up to 4096, int8: 34.5.
 //
 // Every wait is bounded; one that gives up records an error, and the CTA
 // lets its MMAs drain and frees its TMEM before it ends.
@@ -57,7 +67,7 @@ struct ChunkTile {
     static constexpr int KV_HALF = BN * 128, KV_TILE = KV_HALF * (D / 64);
     static constexpr int SMEM_KV = TILES * NP * Q_TILE;
     static constexpr int STAGE = 2 * KV_TILE;
-    static constexpr int AUX = BF ? 3072 : 6144;                                  // barriers and words, below
+    static constexpr int AUX = BF ? 3072 : 6656;                                  // barriers and words, below
     static constexpr int FIT = (232448 - AUX - SMEM_KV) / STAGE;
     static constexpr int STAGES = FIT >= 4 ? 4 : 2;
     static constexpr int SMEM_AUX = SMEM_KV + STAGES * STAGE;
@@ -158,6 +168,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     // while the softmax of that S still runs.
     constexpr int INFO = 4 * STAGES;
     constexpr int NCT = BN / CELL;                 // cells of a tile
+    constexpr int HOLES = 64;
     extern __shared__ __align__(1024) unsigned char base[];
     // Of a tile: K's reference exponents (a quarter of the keys each), V's (a byte per 32 elements), the keys of each cell
     // that some row sees (bit 16: and that lie on a bad page), whether there are any of those. Scales: the tile's
@@ -170,6 +181,12 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         unsigned char qexp[256];
         uint32_t tmem, twin_vref;
         int abort;
+        // Keys that are not finite: 8-bit K or V with a scale of 255, V of BF16 pages where not all rows see all keys. 0
+        // times one would be no 0, so it counts as 0 in the products, and the epilogue makes NaN of the rows that see
+        // it. Cells with such keys in tiles that some row does not see whole (at most 7 tiles of 128 keys), as (first
+        // position, keys); everyone: there is one that all rows see.
+        uint2 hole[HOLES];
+        int n_holes, everyone;
     };
     static_assert(sizeof(Aux) <= T::AUX, "the words behind the operands");
     Aux& aux = *reinterpret_cast<Aux*>(base + T::SMEM_AUX);
@@ -204,6 +221,20 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     const int n_a = twin ? (n_tiles + 1) / 2 : reach_a, n_b = twin ? n_tiles / 2 : has_b ? n_tiles : 0;
     const int n_all = twin ? n_tiles : max(n_a, n_b);
     auto tile_of = [&](int x, int i) { return twin ? 2 * i + x : i; };      // tile x's i-th tile of keys
+    // Keys `keys` of the cell at position key0, of the tile from j0 on, are not finite.
+    auto hole = [&](int j0, int key0, uint32_t keys) {
+        if (!keys) return;
+        const bool edge = j0 + BN - 1 > cw.pos0 + cw.r0 / a.G || (a.window > 0 && j0 <= cw.last - a.window && j0 + BN - 1 >= a.sinks);
+        const int k = edge ? atomicAdd(&aux.n_holes, 1) : HOLES;
+        if (k < HOLES) aux.hole[k] = make_uint2((uint32_t)key0, keys);
+        else aux.everyone = 1;
+    };
+    // Tiles [edge_a, edge_b) of this piece lie at or before the block's first position and, with a window, inside all of its
+    // rows' windows: they need no second look.
+    auto tile_at = [&](int step) { return (step < cw.span.lo ? min(step, cw.span.sunk) : step - cw.span.lo + cw.span.sunk) - t0; };
+    const int edge_a = a.window > 0 ? tile_at(max(0, cw.last - a.window + BN) / BN) : 0;
+    const int edge_b = tile_at(max(0, cw.pos0 + cw.r0 / a.G + 1) / BN);
+    auto on_edge = [&](int j) { return j < edge_a || j >= edge_b; };
 
     // Softmax warps: 16 of their tile's q rows each, D / 8 lanes a row. The first QA of the QSTEPS loads are on their
     // way while barriers and TMEM are set up (asked for after that, four by four, q was there 3 us later).
@@ -282,7 +313,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             mbar_init(&bars[Q_FULL + x], 8);
             mbar_init(&bars[S_FULL + x], 2);      // the products, and the thread that saw the tile's words
             mbar_init(&bars[P_FULL + x], 8);
-            mbar_init(&bars[O_DONE + x], 1);
+            mbar_init(&bars[O_DONE + x], 2);
         }
         mbar_init(&bars[DRAIN], 1);
         for (int s = 0; s < STAGES; ++s) {
@@ -295,6 +326,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         }
         mbar_fence_init();
         s_abort = 0;
+        aux.n_holes = aux.everyone = 0;
     }
     if (warp == CHUNK_MMA_WARP) tmem_alloc(&aux.tmem, 512);
     tc_fence_before();
@@ -341,7 +373,10 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                             for (int k = 0; k < BN / 16; ++k)
                                 mma_bf16_ts(tmem + 256 + x * D, tmem + p_column<BN, NP>(x, k, p), vd + (k * 16 * 128 >> 4), id_o,
                                             i > 0 || p > 0 || k > 0);
-                        if (i + 1 == n_x) mma_commit(&bars[O_DONE + x]);
+                        if (i + 1 == n_x) {
+                            mma_commit(&bars[O_DONE + x]);
+                            mbar_arrive(&bars[O_DONE + x]);
+                        }
                         // Twins: this tile's next S needs the K two tiles on, too late a sign for the V that follows it.
                         if (twin) {
                             mma_commit(&bars[V_EMPTY + j % STAGES]);
@@ -428,29 +463,50 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                 uint32_t km[BN / 32], vm = 0;
                 if (!BF && v == 0) {
                     // K: one reference for 32 keys. V: a reference moves where the tile's largest exponent passes it by
-                    // more than the slack.
-                    #pragma unroll
-                    for (int q = 0; q < BN / 32; ++q) {
-                        uint32_t m = ks[q] & 255u;
+                    // more than the slack. A second time around without scales of 255.
+                    uint32_t top[NB];
+                    #pragma unroll 1
+                    for (;;) {
+                        uint32_t most = 0;
                         #pragma unroll
-                        for (int k = 1; k < NB; ++k) m = max(m, (ks[q] >> (8 * k)) & 255u);
-                        km[q] = __reduce_max_sync(0xffffffffu, m);
+                        for (int q = 0; q < BN / 32; ++q) {
+                            uint32_t m = ks[q] & 255u;
+                            #pragma unroll
+                            for (int k = 1; k < NB; ++k) m = max(m, (ks[q] >> (8 * k)) & 255u);
+                            km[q] = __reduce_max_sync(0xffffffffu, m);
+                            most = max(most, km[q]);
+                        }
+                        #pragma unroll
+                        for (int k = 0; k < NB; ++k) {
+                            uint32_t m = 0;
+                            #pragma unroll
+                            for (int q = 0; q < BN / 32; ++q) m = max(m, (vs[q] >> (8 * k)) & 255u);
+                            top[k] = __reduce_max_sync(0xffffffffu, m);
+                            most = max(most, top[k]);
+                        }
+                        if (most != 255u) break;
+                        #pragma unroll
+                        for (int q = 0; q < BN / 32; ++q) {
+                            const uint32_t k255 = __vcmpeq4(ks[q], 0xffffffffu), v255 = __vcmpeq4(vs[q], 0xffffffffu);
+                            const uint32_t keys = __ballot_sync(0xffffffffu, (k255 | v255) != 0);
+                            ks[q] &= ~k255;
+                            vs[q] &= ~v255;
+                            const int j0 = cw.span.step(t0 + j) * BN;
+                            if (lane < 2) hole(j0, j0 + 32 * q + CELL * lane, (keys >> (CELL * lane)) & 0xffffu);
+                        }
                     }
                     #pragma unroll
                     for (int k = 0; k < NB; ++k) {
-                        uint32_t m = 0;
-                        #pragma unroll
-                        for (int q = 0; q < BN / 32; ++q) m = max(m, (vs[q] >> (8 * k)) & 255u);
-                        m = __reduce_max_sync(0xffffffffu, m);
                         const uint32_t old = (ev >> (8 * k)) & 255u;
-                        vm |= (m > old + SLACK ? m : old) << (8 * k);
+                        vm |= (top[k] > old + SLACK ? top[k] : old) << (8 * k);
                     }
                     ev = vm;
                 }
                 if (lane < NCT) s_need[v][i][lane] = x0.need;
                 if (!BF) {
                     #pragma unroll
-                    for (int q = 0; q < BN / 32; ++q) s_scale[st][v][32 * q + lane] = v ? vs[q] : ks[q];
+                    for (int q = 0; q < BN / 32; ++q)
+                        s_scale[st][v][32 * q + lane] = v ? vs[q] & ~__vcmpeq4(vs[q], 0xffffffffu) : ks[q];
                 }
                 if (v == 0 && lane == 0) {
                     s_bad[i] = bad;
@@ -501,11 +557,22 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                 // Rows that no row of the call sees may hold anything, and 0 times a NaN is no 0: a lane a row.
                 if (lane < KPW) {
                     const int r = sw * KPW + lane;
-                    if (!((need_of(1, j, r) >> (r % CELL)) & 1)) {
+                    const uint32_t at = base_u32 + T::SMEM_KV + (j % STAGES) * T::STAGE + T::KV_TILE + r * 128;
+                    bool no = !((need_of(1, j, r) >> (r % CELL)) & 1), inf = false;
+                    if (on_edge(j)) {
+                        // Nor may a row that is not finite reach rows that do not see it.
+                        #pragma unroll
+                        for (int i = 0; i < D / 8; ++i) inf |= bf16x8_bad(lds128(at + (i >> 3) * T::KV_HALF + ((i + lane) & 7) * 16));
+                        inf = inf && !no;
+                        no |= inf;
+                        const uint32_t keys = __ballot_sync(KPW == 32 ? 0xffffffffu : 0xffffu, inf);
+                        const int j0 = cw.span.step(t0 + j) * BN;
+                        if (lane < KPW / CELL) hole(j0, j0 + sw * KPW + CELL * lane, (keys >> (CELL * lane)) & 0xffffu);
+                    }
+                    if (no) {
                         #pragma unroll
                         for (int i = 0; i < D / 8; ++i)
-                            sts128(base_u32 + T::SMEM_KV + (j % STAGES) * T::STAGE + T::KV_TILE + (i >> 3) * T::KV_HALF + r * 128 + (i & 7) * 16,
-                                   make_uint4(0u, 0u, 0u, 0u));
+                            sts128(at + (i >> 3) * T::KV_HALF + (i & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
                     }
                 }
                 full(V_FULL, j);
@@ -632,6 +699,12 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             mbar_arrive(&bars[bar + j % STAGES]);
             if (twin || k >= (x ? n_a : n_b)) mbar_arrive(&bars[bar + j % STAGES]);
         };
+        // Which of the 32 keys from position k0 on the row sees: at or before its own, inside its window or among the sinks.
+        auto visible = [&](int k0) {
+            const int hi = max(p, -1) - k0, sk = a.sinks - k0;
+            const int lo = (a.window > 0 ? max(max(p, -1) - a.window, -1) : -1) - k0;
+            return bits_below(hi + 1) & (~bits_below(lo + 1) | bits_below(sk));
+        };
         float m_run = -INFINITY, l_run = 0.f, rf = a.scale_log2;
         uint32_t vref = 0;                     // V's references that O is relative to
         for (int i = 0; i < n_x; ++i) {
@@ -653,11 +726,8 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             auto scores = [&](int c0, float (&sc)[32]) {
                 tmem_ld32(s_tm + c0, sc);
                 if (masked) {
-                    // Visible columns as bits: at or before the row's position, inside its window or among the
-                    // sinks, and really there. Two instructions a column then.
-                    const int hi = max(p, -1) - j0 - c0, sk = a.sinks - j0 - c0;
-                    const int lo = (a.window > 0 ? max(max(p, -1) - a.window, -1) : -1) - j0 - c0;
-                    uint32_t see = bits_below(hi + 1) & (~bits_below(lo + 1) | bits_below(sk));
+                    // Visible columns as bits; two instructions a column then.
+                    uint32_t see = visible(j0 + c0);
                     if (bad) see &= (s_need[0][s][c0 / 16] & 0xffffu) | s_need[0][s][c0 / 16 + 1] << 16;
                     #pragma unroll
                     for (int c = 0; c < 32; ++c)
@@ -667,7 +737,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             // The factor of a quarter of the keys; never 0, a masked score is -inf times it.
             auto factor = [&](int k) {
                 const uint32_t e = BF ? 0u : s_km[s][k];
-                return BF ? rf : fmaxf(rf * (e == 255u ? INFINITY : __uint_as_float(e << 23)), 1.2e-38f);
+                return BF ? rf : fmaxf(rf * __uint_as_float(e << 23), 1.2e-38f);
             };
             constexpr int QN = BN / 4 < 32 ? BN / 4 : 32;             // columns under one factor
             auto half_max = [&](int h) {
@@ -757,6 +827,12 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
         if (ok && n_x > 0 && !twin && (warp & 7) == 0 && lane == 0) pass_on(V_EMPTY, n_x - 1);
         if (ok && (x ? n_a : n_b) > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars[O_DONE + (x ^ 1)], 0));
         ok = __all_sync(0xffffffffu, ok && !aborted());
+        if (n_x > 0 && (*(volatile int*)&aux.n_holes | *(volatile int*)&aux.everyone)) {
+            bool sees_one = *(volatile int*)&aux.everyone != 0;
+            for (int k = 0; k < min(HOLES, *(volatile int*)&aux.n_holes); ++k)
+                sees_one |= (visible((int)aux.hole[k].x) & aux.hole[k].y) != 0;
+            if (sees_one) l_run = __uint_as_float(0x7fc00000u);
+        }
         // Each thread's maximum and sum: [tile][half][row], in the place of q.
         float2* s_ml = reinterpret_cast<float2*>(base);
         asm volatile("bar.sync 9, 512;" ::: "memory");             // all 16 warps are past the products
@@ -796,7 +872,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                 }
                 auto v_scale_of = [&](uint32_t ref) {
                     const uint32_t e = (ref >> (8 * c)) & 255u;
-                    return BF ? 1.0f : e == 255u ? INFINITY : __uint_as_float(e << 23);
+                    return BF ? 1.0f : __uint_as_float(e << 23);
                 };
                 const float ga = inv * f_a * (n_x > 0 ? v_scale_of(vref) : 1.0f);
                 #pragma unroll

@@ -29,6 +29,15 @@
 // The running maximum moves only when some score passes it by 2^8 (a warp
 // vote), so most cells need no reduction over the keys; p is held times 2^7
 // so that small weights stay above F16's subnormals.
+//
+// What bounds it: the instructions that turn codes into numbers (an SM streams
+// 39 GB/s of 8-bit cells with 16 warps, 5.7 TB/s in all, against 6.5 that HBM
+// gives; BF16 cells 6.3 TB/s), then how evenly the SMs are filled: work comes in CTAs of one
+// piece of one sequence's keys, with about 5 us before and after its stream.
+// Measured (us; with the join): 16 sequences of 32768 keys, 64 / 8 heads, int8: 219 (5.07 TB/s); 64 ragged
+// ones up to 4096, 32 / 8 heads, E4M3, F32 rows: 85 (3.3); 16 with a window of
+// 4096 of 32768, BF16 pages, F32 rows: 47 (5.1); one of 4096, E4M3: 11.9 (latency: a launch, page
+// ids, keys, the join).
 #pragma once
 #include <cuda_fp16.h>
 
@@ -116,7 +125,7 @@ PCU_DEV void split_parts(float lo, float hi, uint32_t (&p)[N]) {
     }
 }
 
-// 2^(e - ref) of scale bytes, as F32; at or below 2^-127 it is 0. e - ref <= 127.
+// 2^(e - ref) of scale bytes, as F32; at or below 2^-127 it is 0, infinite for e - ref = 128, no more.
 PCU_DEV float rel_scale(int e, int ref) { return __uint_as_float((uint32_t)max(e - ref + 127, 0) << 23); }
 
 PCU_DEV uint32_t e4m3x2_f16x2(uint32_t pair) {
@@ -334,7 +343,7 @@ pages_decode_kernel(const AttnArgs a) {
             cur = nxt;
             nxt = look_up(i + 32);
         }
-        const uint32_t need = (uint32_t)__shfl_sync(0xffffffffu, cur.need, i & 31);
+        uint32_t need = (uint32_t)__shfl_sync(0xffffffffu, cur.need, i & 31);
         const int j0 = span.step(e0 + warp + i * W) * CELL;
         cp_async_wait<STAGES - 1>();
         __syncwarp();
@@ -352,8 +361,11 @@ pages_decode_kernel(const AttnArgs a) {
                         x1 = (need >> (g + 8)) & 1 ? x1 : 0;
                     }
                     if (__any_sync(0xffffffffu, max(x0, x1) > ek + SLACK)) {
-                        ek = __reduce_max_sync(0xffffffffu, max(x0, x1));
-                        const float f = ek == 255 ? INFINITY : __uint_as_float((uint32_t)ek << 23);
+                        // A key with a block of scale 255 gets infinite factors, so NaN scores, and moves no reference.
+                        ek = max(ek, __reduce_max_sync(0xffffffffu, max(x0 == 255 ? 0 : x0, x1 == 255 ? 0 : x1)));
+                        x0 = x0 == 255 ? ek + 128 : x0;
+                        x1 = x1 == 255 ? ek + 128 : x1;
+                        const float f = __uint_as_float((uint32_t)ek << 23);
                         #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             fc[k] = fmaxf(fc0[k] * f, 1.2e-38f);      // never 0: a masked score is -inf * fc
@@ -396,10 +408,35 @@ pages_decode_kernel(const AttnArgs a) {
             for (int k = 0; k < 4; ++k) s[k] = sp[0][k] + sp[1][k];
             if (need != 0xffffu || j0 + CELL - 1 > pos0 ||
                 (a.window > 0 && j0 <= kv - 1 - a.window && j0 + CELL - 1 >= a.sinks)) {
+                // Not all rows see all of the cell: a V row that is not finite must not reach those that do not see it, and
+                // 0 times it is no 0. The rows that see it get a NaN score, and it counts as not needed: 0.
+                bool bad[2] = {false, false};
+                #pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = g + 8 * h;
+                    if (BF) {
+                        #pragma unroll
+                        for (int j = 0; j < T::KCH; ++j)
+                            bad[h] |= bf16x8_bad(*reinterpret_cast<const uint4*>(cell + v_row(KV, D, r) + T::at(r, T::k_chunk(t, j)) * 16));
+                        bad[h] |= __shfl_xor_sync(0xffffffffu, (int)bad[h], 1) != 0;
+                        bad[h] |= __shfl_xor_sync(0xffffffffu, (int)bad[h], 2) != 0;
+                    } else {
+                        const uint32_t e = D == 128 ? *reinterpret_cast<const uint32_t*>(cell + v_scale(D, r))
+                                                    : *reinterpret_cast<const uint16_t*>(cell + v_scale(D, r));
+                        bad[h] = __vcmpeq4(e, 0xffffffffu) != 0;
+                    }
+                    bad[h] = bad[h] && ((need >> r) & 1);
+                }
                 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int r = g + 8 * (k >> 1);
                     if (!((need >> r) & 1) || !sees(pc[k & 1], j0 + r, a.window, a.sinks)) s[k] = -INFINITY;
+                    else if (bad[k >> 1]) s[k] = __uint_as_float(0x7fc00000u);
+                }
+                const uint32_t v0 = __ballot_sync(0xffffffffu, bad[0]), v1 = __ballot_sync(0xffffffffu, bad[1]);     // bit 4 g
+                if (v0 | v1) {
+                    #pragma unroll
+                    for (int k = 0; k < 16; ++k) need &= ~((((k < 8 ? v0 : v1) >> (4 * (k & 7))) & 1u) << k);
                 }
             }
             const float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
@@ -445,6 +482,11 @@ pages_decode_kernel(const AttnArgs a) {
                     #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         x[k] = *reinterpret_cast<const uint4*>(cell + v_row(KV, D, rk[k]) + T::at(rk[k], g + 8 * half) * 16);
+                    if (need != 0xffffu) {
+                        #pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (!((need >> rk[k]) & 1)) x[k] = make_uint4(0u, 0u, 0u, 0u);
+                    }
                     #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const uint32_t x0 = (&x[0].x)[e], x1 = (&x[1].x)[e], x2 = (&x[2].x)[e], x3 = (&x[3].x)[e];
@@ -518,7 +560,7 @@ pages_decode_kernel(const AttnArgs a) {
     cp_async_wait<0>();
 
     // Join the warps: partial (m, l, O) of each through shared memory.
-    const float vf = BF ? 1.0f : ev == 255 ? INFINITY : __uint_as_float((uint32_t)ev << 23);
+    const float vf = BF ? 1.0f : scale_f32((uint32_t)ev);
     #pragma unroll
     for (int i = 0; i < 2; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);

@@ -566,3 +566,43 @@ def test_chunks_of_ragged_contexts(rows, lens, most):
     first = _check_attn(B, 4, rows, q=q, batch=batch)
     assert torch.equal(first, _check_attn(B, 4, rows, q=q, batch=batch))
     _check_attn(B, 4, rows, 300, 20, q=q, batch=batch)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "i8", "e4m3"])
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G,n", [(1, 5), (2, 4), (4, 40), (8, 60), (1, 200)])
+@pytest.mark.parametrize("which,window", [("k", 0), ("v", 0), ("k", 3), ("v", 3)])
+def test_rows_that_do_not_see_a_number_that_is_not_finite(kv, rows, D, G, n, which, window):
+    """A NaN or an infinity in k or v at a position that some rows of the call see and others do not: those that do not
+    get their numbers, those that do get none. Without a window it is the last row but two of the call, with one the row
+    before the call."""
+    B = R.Batch(kv, 2, D, 16, [300, 77], [n, 3], 71)
+    cache, batch = _cache(B), _batch(B)
+    at = 300 - 3 if not window else 300 - n - 1
+    k, v = torch.zeros((1, 2, D), device=DEV), torch.zeros((1, 2, D), device=DEV)
+    k[0, 0], v[0, 0] = B.k[0][0, at].float(), B.v[0][0, at].float()
+    k[0, 1], v[0, 1] = B.k[0][1, at].float(), B.v[0][1, at].float()
+    (k if which == "k" else v)[0, 1, D - 7] = float("inf") if which == "v" and not window else float("nan")
+    one = PageBatch(torch.tensor([at + 1], dtype=torch.int32, device=DEV), B.tensors()[1][:1].contiguous())
+    cache.append_dev(0, one, k, v)
+    q = B.randn(B.n_tok, 2 * G, D).to(R.ROWS[rows])
+    out = torch.full_like(q, 7.0)
+    cache.attn_dev(0, batch, q, out, window=window)
+    cache.sync()
+    for b, t in ((0, 0), (1, n)):
+        m = B.q_len[b]
+        ref, mass, size = R.attend(q[t:t + m], B.k[b], B.v[b], B.positions(b), window, 0)
+        tol = R.attn_bound(mass, size, ref, rows, B.kv_len[b], rows == "bf16")
+        sees = torch.tensor([b == 0 and at <= p and (not window or at > p - window) for p in B.positions(b)], device=DEV)
+        good = torch.ones_like(ref, dtype=torch.bool)
+        good[sees, G:] = False                                       # KV head 1's query heads
+        err = (out[t:t + m].double() - ref).abs()
+        assert torch.isfinite(out[t:t + m][good]).all()
+        assert (err[good] <= tol[good]).all(), f"{float((err / tol)[good].max()):.2f} of the bound"
+        if b == 0:
+            assert 0 < int(sees.sum()) < m
+            bad = out[:m][sees, G:]
+            assert (~torch.isfinite(bad)).any(-1).all()
+            if which == "k":
+                assert torch.isnan(bad).all()

@@ -492,7 +492,7 @@ PICKLE_CUDA_API int  pickle_cuda_pages_read_dev(const pickle_cuda_pages_t* pages
  * Pages that no row of the call can see are never touched (their table
  * entries may be stale). A row that sees no key gives zeros. Keys on a page
  * outside the pool are left out and recorded in the error word. A k or v
- * element that is not finite makes the rows that see it NaN (of a v element
+ * element that is not finite makes the rows that see it so (of a v element
  * the whole row or the elements next to it) and no other row.
  * The answers depend on the batch's bounds in their last bits only, and are
  * the same bits for the same call.

@@ -60,6 +60,9 @@ template <int KV, int D, int ROWS>
 struct ChunkTile {
     static constexpr bool BF = KV == BF16;
     static constexpr int NP = ROWS == PICKLE_CUDA_ROW_BF16 ? 1 : BF ? 3 : 2;      // operands a q or p is split into
+    // The tensor cores cut their sums off instead of rounding them, always towards 0, once a product: the small parts of
+    // P get sums of their own where TMEM has room (1.3e-6 without, D = 64 after 1000 keys).
+    static constexpr bool APART = NP == 2 && D == 64;
     static constexpr int TILES = NP == 3 && D == 128 ? 1 : 2;                      // 128-row tiles
     static constexpr int BN = NP > 1 && D == 128 ? 64 : 128;                       // keys of a tile
     static constexpr int ROWS_CTA = TILES * 128;
@@ -371,8 +374,8 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                         for (int p = 0; p < NP; ++p)
                             #pragma unroll
                             for (int k = 0; k < BN / 16; ++k)
-                                mma_bf16_ts(tmem + 256 + x * D, tmem + p_column<BN, NP>(x, k, p), vd + (k * 16 * 128 >> 4), id_o,
-                                            i > 0 || p > 0 || k > 0);
+                                mma_bf16_ts(tmem + 256 + x * D + (T::APART && p > 0 ? 128 : 0), tmem + p_column<BN, NP>(x, k, p),
+                                            vd + (k * 16 * 128 >> 4), id_o, i > 0 || (p > 0 && !T::APART) || k > 0);
                         if (i + 1 == n_x) {
                             mma_commit(&bars[O_DONE + x]);
                             mbar_arrive(&bars[O_DONE + x]);
@@ -781,13 +784,15 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
             if (i > 0 && __any_sync(0xffffffffu, grow || vnow != vref)) {
                 // This half's columns of O. S_FULL_X(i) implies PV_X(i - 1) is complete, and PV_X(i) waits for P_FULL.
                 #pragma unroll 1
-                for (int c = hf * (D / 64); c < (hf + 1) * (D / 64); ++c) {
+                for (int y = hf * (D / 64); y < (hf + 1) * (D / 64) + (T::APART ? 1 : 0); ++y) {
+                    // (Apart: one step for the large part, one for the small.)
+                    const int c = T::APART ? hf : y, at = c * 32 + (T::APART && y > hf ? 128 : 0);
                     float o[32];
-                    tmem_ld32(o_tm + c * 32, o);
+                    tmem_ld32(o_tm + at, o);
                     const float g = BF ? alpha : alpha * rel_scale((vref >> (8 * c)) & 255, (vnow >> (8 * c)) & 255);
                     #pragma unroll
                     for (int k = 0; k < 32; ++k) o[k] *= g;
-                    tmem_st32(o_tm + c * 32, o);
+                    tmem_st32(o_tm + at, o);
                 }
             }
             float2 sm2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -866,6 +871,12 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                 float o[32];
                 if (n_x > 0) {
                     tmem_ld32(o_tm + c * 32, o);
+                    if (T::APART) {
+                        float small[32];
+                        tmem_ld32(o_tm + 128 + c * 32, small);
+                        #pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] += small[k];
+                    }
                 } else {
                     #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0.f;
@@ -880,6 +891,12 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
                 if (twin) {
                     float ob[32];
                     tmem_ld32(o_tm + D + c * 32, ob);            // O_B: the same lanes, the next columns
+                    if (T::APART) {
+                        float small[32];
+                        tmem_ld32(o_tm + D + 128 + c * 32, small);
+                        #pragma unroll
+                        for (int k = 0; k < 32; ++k) ob[k] += small[k];
+                    }
                     const float gb = inv * f_b * v_scale_of(vref_b);
                     #pragma unroll
                     for (int k = 0; k < 32; ++k) o[k] = fmaf(ob[k], gb, o[k]);

@@ -10,7 +10,8 @@
 //               layout (128-byte swizzle), 8-bit pages with bulk copies of the
 //               codes into the place of their operands, and their scales;
 //   warps 16-19 turn a tile's codes in place into 16-bit operands (K-major K,
-//               MN-major V); of BF16 pages they only clear V rows that no row sees;
+//               MN-major V); of BF16 pages they only clear V rows that no row
+//               sees, or that are not finite and not seen by all;
 //   warp 20     one lane issues tcgen05.mma: S_X = Q_X K^T, O_X += P_X V,
 //               P_X read from TMEM, in the order PV_A, S_A, PV_B, S_B so that one
 //               tile's softmax runs under the other's products;
@@ -40,9 +41,9 @@
 // operands, tiles of 64 keys). Twins, 128 rows or fewer: 1.5 and 2.0. An item of 256 rows adds about 10 us
 // that nothing hides, one CTA filling an SM: page ids and q (3 us), the first
 // keys and softmax (5 us), the epilogue (3 us).
-// Measured (us): 2048 tokens on 8192, 32 / 8 heads, E4M3: 377 (820 TFLOP/s); 4 prompts of 2048, 32 / 32 heads,
-// BF16: 228 (604); 2 ragged ones up to 4001, window 1000, F32, D = 64, int8: 113;
-// 8 x 16 tokens on ragged contexts up to 4096, int8: 34.5.
+// Measured (us): 2048 tokens on 8192, 32 / 8 heads, E4M3: 384 (806 TFLOP/s); 4 prompts of 2048, 32 / 32 heads,
+// BF16: 236 (583); 2 ragged ones up to 4001, window 1000, F32, D = 64, int8: 118;
+// 8 x 16 tokens on ragged contexts up to 4096, int8: 35.
 //
 // Every wait is bounded; one that gives up records an error, and the CTA
 // lets its MMAs drain and frees its TMEM before it ends.

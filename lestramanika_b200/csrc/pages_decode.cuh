@@ -34,9 +34,9 @@
 // 39 GB/s of 8-bit cells with 16 warps, 5.7 TB/s in all, against 6.5 that HBM
 // gives; BF16 cells 6.3 TB/s), then how evenly the SMs are filled: work comes in CTAs of one
 // piece of one sequence's keys, with about 5 us before and after its stream.
-// Measured (us; with the join): 16 sequences of 32768 keys, 64 / 8 heads, int8: 219 (5.07 TB/s); 64 ragged
-// ones up to 4096, 32 / 8 heads, E4M3, F32 rows: 85 (3.3); 16 with a window of
-// 4096 of 32768, BF16 pages, F32 rows: 47 (5.1); one of 4096, E4M3: 11.9 (latency: a launch, page
+// Measured (us; with the join): 16 sequences of 32768 keys, 64 / 8 heads, int8: 217 (5.1 TB/s); 64 ragged
+// ones up to 4096, 32 / 8 heads, E4M3, F32 rows: 88 (3.2); 16 with a window of
+// 4096 of 32768, BF16 pages, F32 rows: 48 (5.0); one of 4096, E4M3: 12.4 (latency: a launch, page
 // ids, keys, the join).
 #pragma once
 #include <cuda_fp16.h>

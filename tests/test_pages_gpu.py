@@ -577,9 +577,22 @@ def test_rows_that_do_not_see_a_number_that_is_not_finite(kv, rows, D, G, n, whi
     """A NaN or an infinity in k or v at a position that some rows of the call see and others do not: those that do not
     get their numbers, those that do get none. Without a window it is the last row but two of the call, with one the row
     before the call."""
-    B = R.Batch(kv, 2, D, 16, [300, 77], [n, 3], 71)
+    _check_unseen(kv, rows, D, G, n, which, window, 300)
+
+
+@pytest.mark.parametrize("kv,rows", [("bf16", "f32"), ("bf16", "bf16"), ("i8", "bf16"), ("e4m3", "f32")])
+@pytest.mark.parametrize("G,n", [(2, 3), (4, 20)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_numbers_that_are_not_finite_in_split_contexts(kv, rows, G, n, which):
+    """The same where the keys are cut into pieces that are joined."""
+    _check_unseen(kv, rows, 128, G, n, which, 0, 9000)
+
+
+def _check_unseen(kv, rows, D, G, n, which, window, length):
+    B = R.Batch(kv, 2, D, 16, [length, 77], [n, 3], 71)
     cache, batch = _cache(B), _batch(B)
-    at = 300 - 3 if not window else 300 - n - 1
+    assert length < 9000 or cache.attn_workspace(batch, 2 * G, 0 if rows == "f32" else 1, window) > 0
+    at = length - (2 if n < 5 else 3) if not window else length - n - 1
     k, v = torch.zeros((1, 2, D), device=DEV), torch.zeros((1, 2, D), device=DEV)
     k[0, 0], v[0, 0] = B.k[0][0, at].float(), B.v[0][0, at].float()
     k[0, 1], v[0, 1] = B.k[0][1, at].float(), B.v[0][1, at].float()

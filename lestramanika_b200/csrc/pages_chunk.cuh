@@ -71,7 +71,7 @@ struct ChunkTile {
     static constexpr int KV_HALF = BN * 128, KV_TILE = KV_HALF * (D / 64);
     static constexpr int SMEM_KV = TILES * NP * Q_TILE;
     static constexpr int STAGE = 2 * KV_TILE;
-    static constexpr int AUX = BF ? 3072 : 6656;                                  // barriers and words, below
+    static constexpr int AUX = BF ? 3040 : 6656;                                  // barriers and words, below
     static constexpr int FIT = (232448 - AUX - SMEM_KV) / STAGE;
     static constexpr int STAGES = FIT >= 4 ? 4 : 2;
     static constexpr int SMEM_AUX = SMEM_KV + STAGES * STAGE;

@@ -53,8 +53,8 @@ struct DecodeTile {
     static constexpr int KCH = CH / 4;                // chunks of a K row that a lane takes
     static constexpr int CELLB = cell_bytes(KV, D);
     // 8-bit: 16 warps an SM with 12 KB of ring each (203 KB in all), in four CTAs: in two of eight warps, what a CTA does
-    // before its first and after its last cell is hidden less (16 sequences of 32768, 8 heads: 232 us instead of 199; 64
-    // ragged ones up to 4096: 89 instead of 81). BF16 cells are twice as large and cheaper to use: 12 warps with 16 KB.
+    // before its first and after its last cell is hidden less (16 sequences of 32768, 8 heads: 232 us instead of 219; 64
+    // ragged ones up to 4096: 89 instead of 85). BF16 cells are twice as large and cheaper to use: 12 warps with 16 KB.
     static constexpr int WARPS = 4;
     static constexpr int CTAS = KV == BF16 ? 3 : 4;
     static constexpr int STAGES = (KV == BF16 ? 2 : 3) * 128 / D;

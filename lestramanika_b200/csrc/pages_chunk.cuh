@@ -23,8 +23,8 @@
 // 8-bit codes become F16 numbers code * 2^(e - E), exact but for elements
 // 2^-24 below the reference: K has one E for 32 keys of a tile, which the
 // softmax undoes in the factor it applies anyway;
-// V has a running one per 32 elements, 2^7 of slack below F16's largest number, and
-// moving it rescales O. Elements keep the order that is cheapest to unpack;
+// V has a running one per 32 elements, which a tile may pass by 2^5 (int8) or 2^7 (E4M3)
+// before it moves, and moving it rescales O. Elements keep the order that is cheapest to unpack;
 // Q is written, and O read, in the same order. BF16 pages are copied and
 // multiplied as they are.
 //
@@ -163,7 +163,7 @@ pages_chunk_kernel(const __grid_constant__ CUtensorMap tm, const AttnArgs a) {
     constexpr bool BF = T::BF;
     constexpr int NP = T::NP, BN = T::BN, STAGES = T::STAGES, NB = D / 32;
     constexpr float P_SHIFT = BF ? 0.f : 7.f, GROW = 8.f;
-    constexpr int SLACK = 7;
+    constexpr int SLACK = Slack<KV>::value;
     enum { Q_FULL = 0, S_FULL = 2, P_FULL = 4, O_DONE = 6, DRAIN = 8, K_FULL = 9, K_EMPTY = K_FULL + STAGES,
            V_FULL = K_EMPTY + STAGES, V_EMPTY = V_FULL + STAGES, RAW_K = V_EMPTY + STAGES, RAW_V = RAW_K + STAGES,
            N_BARS = RAW_V + STAGES };

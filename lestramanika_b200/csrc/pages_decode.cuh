@@ -145,6 +145,16 @@ PCU_DEV void add_products(float (&o)[4], uint32_t a0, uint32_t a1, uint32_t a2, 
 // 2^(e - ref) of scale bytes, as F32; at or below 2^-127 it is 0, infinite for e - ref = 128, no more.
 PCU_DEV float rel_scale(int e, int ref) { return __uint_as_float((uint32_t)max(e - ref + 127, 0) << 23); }
 
+// How far a block's exponent may pass the reference that its codes are made F16 numbers under. E4M3: code * 2^SLACK has
+// to be an F16 number. I8: so has 1152 * 2^SLACK, which codes_row and codes_pair take off again. And 255, the scale of
+// blocks that are not finite, has to pass the largest reference that finite ones make by more (i8: 249, E4M3: 247).
+template <int KV>
+struct Slack {
+    static constexpr int value = KV == I8 ? 5 : 7;
+    static_assert((KV == I8 ? 1152 : 448) * (1 << value) <= 65504, "numbers that codes are unpacked through are finite in F16");
+    static_assert((KV == I8 ? 249 : 247) + value < 255, "a scale of 255 is noticed");
+};
+
 PCU_DEV uint32_t e4m3x2_f16x2(uint32_t pair) {
     uint32_t h;
     asm("{\n\t.reg .b16 p, u;\n\tmov.b32 {p, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, p;\n\t}" : "=r"(h) : "r"(pair));
@@ -159,8 +169,8 @@ PCU_DEV uint32_t i8_magic(uint32_t x) {
     return y;
 }
 
-// Four consecutive codes of a row, times f (both halves): the pairs of one k-step. I8: elements (0, 2), (1, 3);
-// E4M3: (0, 1), (2, 3). c = -1152 f; the fused product is exact.
+// Four consecutive codes of a row, times f (both halves, at most 2^SLACK): the pairs of one k-step. I8: elements (0, 2),
+// (1, 3); E4M3: (0, 1), (2, 3). c = -1152 f; the fused product is exact.
 template <int KV>
 PCU_DEV void codes_row(uint32_t w, uint32_t f, uint32_t c, uint32_t& p0, uint32_t& p1) {
     if (KV == I8) {
@@ -237,7 +247,7 @@ pages_decode_kernel(const AttnArgs a) {
     constexpr int QP = !F32 ? 1 : BF ? 3 : 2, PP = BF ? (F32 ? 3 : 2) : (F32 ? 2 : 1);
     constexpr int W = T::WARPS, STAGES = T::STAGES;
     constexpr int KS = D / 16, MT = D / 16;
-    constexpr int SLACK = 7;              // how far an exponent may pass its reference: 448 * 2^7 is below F16's largest
+    constexpr int SLACK = Slack<KV>::value;
     constexpr float P_SHIFT = BF ? 0.f : 7.f, GROW = 8.f;
     extern __shared__ __align__(128) unsigned char smem[];
     const View& w = a.w;

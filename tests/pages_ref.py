@@ -103,8 +103,19 @@ def attn_bound(mass, size, out, rows, n_keys, rounded_p):
     return tol
 
 
+def held_weights(k, v, pos, window, sinks):
+    """What the 8-bit pages' weights held as F16 add to the bound, [n][1][D] over a KV head's rows of k, v [m][D]: a
+    weight is held as 2^7 or more times itself over the row's largest, so the rounding to F16's smallest step, 2^-24,
+    moves it by at most 2^-25 / 2^7, whatever is far below the row's largest weight included."""
+    see = visible(pos, k.shape[0], window, sinks, v.device).double()
+    return (2.0 ** -32 * (see @ v.abs()))[:, None]
+
+
 class Batch:
-    """A random pool and ragged batch. Rows that no sequence owns are 255 bytes: NaN codes and NaN scales."""
+    """A random pool and ragged batch. Rows that no sequence owns are 255 bytes: NaN codes and NaN scales.
+
+    amp: what the N(0, 1) rows are multiplied by, a number or a function of (sequence, which, length) that gives a
+    tensor for [HK][length][D], which being 0 for K and 1 for V."""
 
     def __init__(self, kv, HK, D, page, kv_len, q_len, seed, device="cuda:0", spare=3, fill=True, amp=1.0):
         self.kv, self.HK, self.D, self.page = kv, HK, D, page
@@ -125,7 +136,7 @@ class Batch:
         for b, m in enumerate(kv_len):
             pair = []
             for which in (0, 1):
-                x = torch.randn((HK, m, D), generator=g) * amp
+                x = torch.randn((HK, m, D), generator=g) * (amp(b, which, m) if callable(amp) else amp)
                 val, codes, scale = quantise(x, kv)
                 pair.append(val.to(self.dev))
                 if fill and m:

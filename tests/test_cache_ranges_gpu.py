@@ -1,0 +1,101 @@
+"""Attention over pages whose rows differ in magnitude: along the sequence, between blocks of 32, and far apart."""
+import pytest
+import torch
+
+import pages_ref as R
+from lestramanika_b200.pages import KVPages, PageBatch
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+# Rows of two sequences and query heads of a KV head: the kernel for few rows with one token and with several; the one
+# for many with both its tiles on the same rows, and with two blocks of rows.
+CALLS = {"one": (4, [1, 1]), "few": (2, [4, 3]), "twin": (2, [40, 5]), "many": (4, [70, 5])}
+FORMS = [(kv, rows, D, call) for kv in ("i8", "e4m3", "bf16") for rows in ("f32", "bf16") for D in (64, 128) for call in CALLS]
+
+
+@pytest.fixture(params=["1", "2", "0"], ids=["whole", "halves", "planned"])
+def pieces(request, monkeypatch):
+    """How many pieces a sequence's keys are cut into: a piece finds its own magnitudes, and the planned ones are short."""
+    monkeypatch.setenv("PICKLE_CUDA_PAGES_SPLITS", request.param)
+
+
+def _amp(pattern, f, D):
+    """2^0 to 2^f over positions or blocks, as a function for R.Batch."""
+    def of(b, which, m):
+        j = torch.arange(m, dtype=torch.float32)
+        one, top = torch.ones(m), torch.full((m,), 2.0 ** f)
+        col = {"rise": torch.where(j < m // 2, one, top), "fall": torch.where(j < m // 2, top, one),
+               "drift up": 2.0 ** (f * j / max(1, m - 1)), "drift down": 2.0 ** (f * (1 - j / max(1, m - 1))),
+               "first": torch.where(j < 4, one, top), "block": one}[pattern]
+        x = col[:, None].expand(m, D).clone()
+        if pattern == "block":
+            x[:, D - 32:] *= 2.0 ** f
+        return x
+    return of
+
+
+def _check(B, G, rows, q, extra=None, window=0, sinks=0):
+    """attn_dev of q against 64 bits, with R.attn_bound, the held weights of 8-bit pages and `extra`."""
+    kv, table, start = B.tensors()
+    cache = KVPages(R.KV[B.kv], B.n_pages, B.page, B.HK, B.D, pools=[B.pool])
+    out = torch.full_like(q, 7.0)
+    cache.attn_dev(0, PageBatch(kv, table, q_start=start), q, out, window=window, sinks=sinks)
+    cache.sync()
+    assert torch.isfinite(out).all()
+    for b, (n, m) in enumerate(zip(B.q_len, B.kv_len)):
+        t = B.start[b]
+        ref, mass, size = R.attend(q[t:t + n], B.k[b], B.v[b], B.positions(b), window, sinks)
+        tol = R.attn_bound(mass, size, ref, rows, m, rows == "bf16")
+        if B.kv != "bf16":
+            held = [R.held_weights(B.k[b][h], B.v[b][h], B.positions(b), window, sinks) for h in range(B.HK)]
+            tol = tol + torch.cat([x.expand(-1, G, -1) for x in held], 1)
+        if extra is not None:
+            tol = tol + extra(b, mass)
+        err = (out[t:t + n].double() - ref).abs()
+        assert (err <= tol).all(), f"sequence {b}: {float((err / tol).max()):.2f} of the bound"
+
+
+@pytest.mark.parametrize("kv,rows,D,call", FORMS)
+@pytest.mark.parametrize("pattern", ["rise", "fall", "drift up", "drift down", "first", "block"])
+def test_magnitudes_that_differ(pattern, kv, rows, D, call, monkeypatch):
+    """Steps of every power of two up to 2^12, over which every code of both 8-bit types is exact in the products. One
+    piece: what follows a step is taken with what came before it."""
+    monkeypatch.setenv("PICKLE_CUDA_PAGES_SPLITS", "1")
+    G, q_len = CALLS[call]
+    for f in range(13) if pattern in ("rise", "fall") else (5, 6, 7, 12):
+        B = R.Batch(kv, 1, D, 16, [260, 37], q_len, 81 + f, amp=_amp(pattern, f, D))
+        _check(B, G, rows, (B.randn(B.n_tok, G, D) * 2.0 ** -f).to(R.ROWS[rows]))
+
+
+@pytest.mark.parametrize("kv,rows,D", [("i8", "f32", 128), ("i8", "bf16", 64), ("e4m3", "f32", 64), ("e4m3", "bf16", 128),
+                                       ("bf16", "f32", 128)])
+@pytest.mark.parametrize("call", ["one", "twin"])
+@pytest.mark.parametrize("pattern", ["rise", "fall", "drift up"])
+def test_magnitudes_that_differ_between_pieces(pattern, call, kv, rows, D, pieces):
+    """Long contexts, whole and cut into pieces that find different magnitudes and are joined."""
+    G, q_len = CALLS[call]
+    for f in (6, 12):
+        B = R.Batch(kv, 1, D, 64, [2501, 5], q_len, 91 + f, amp=_amp(pattern, f, D))
+        _check(B, G, rows, (B.randn(B.n_tok, G, D) * 2.0 ** -f).to(R.ROWS[rows]))
+
+
+@pytest.mark.parametrize("kv", ["i8", "e4m3"])
+@pytest.mark.parametrize("call", CALLS)
+def test_a_key_that_is_not_finite_among_the_largest(kv, call, pieces):
+    """Scales at the top of their range, and one of 255 behind them, which all rows see."""
+    G, q_len = CALLS[call]
+    B = R.Batch(kv, 1, 128, 16, [260, 37], q_len, 99, amp=lambda b, which, m: 1.0 if which else 2.0 ** 124)
+    cache = KVPages(R.KV[kv], B.n_pages, 16, 1, 128, pools=[B.pool])
+    kv_len, table, start = B.tensors()
+    k, v = torch.full((1, 1, 128), 2.0 ** 127, device=DEV), torch.ones((1, 1, 128), device=DEV)
+    for at in (48, 49, 179):                        # cells 3 and 11: the same warp's first and last, where four share them
+        if at == 179:
+            k[0, 0, 70] = float("nan")
+        one = PageBatch(torch.tensor([at + 1], dtype=torch.int32, device=DEV), table[:1].contiguous())
+        cache.append_dev(0, one, k, v)
+    q = B.randn(B.n_tok, G, 128) * 2.0 ** -120
+    out = torch.empty_like(q)
+    cache.attn_dev(0, PageBatch(kv_len, table, q_start=start), q, out)
+    cache.sync()
+    assert torch.isnan(out[:q_len[0]]).all()

@@ -272,23 +272,27 @@ class KVPages:
         with self._torch.cuda.device(self.device):
             return self._lib.pickle_cuda_pages_workspace(self._refs[0], batch._ref, n_heads, row_type, window, sinks)
 
+    def _stream(self, stream):
+        """The torch stream that a call's `stream` stands for. (ExternalStream makes a new stream of handle 0.)"""
+        cuda = self._torch.cuda
+        if stream is None:
+            return cuda.current_stream(self._dev)
+        if not isinstance(stream, int):
+            return stream
+        return cuda.ExternalStream(stream, device=self._dev) if stream else cuda.default_stream(self._dev)
+
     def _scratch(self, nbytes, stream):
         """Bytes from torch's allocator, tied to the stream that uses them."""
         torch = self._torch
         if stream is None:
             return torch.empty(nbytes, dtype=torch.uint8, device=self._dev)
-        s = torch.cuda.ExternalStream(stream, device=self._dev) if isinstance(stream, int) else stream
-        with torch.cuda.stream(s):
+        with torch.cuda.stream(self._stream(stream)):
             return torch.empty(nbytes, dtype=torch.uint8, device=self._dev)
 
     def sync(self, stream=None):
         """Wait for the stream's work and raise PICKLE_ERR_DEVICE for a device-side error recorded since the last."""
         torch = self._torch
-        if stream is None:
-            torch.cuda.current_stream(self._dev).synchronize()
-        else:
-            s = torch.cuda.ExternalStream(stream, device=self._dev) if isinstance(stream, int) else stream
-            s.synchronize()
+        self._stream(stream).synchronize()
         code = int(self.err.item())
         if code:
             self.err.zero_()

@@ -1,0 +1,74 @@
+"""Streams of the paged KV cache's calls without a GPU: stand-ins for torch's streams record what would be done."""
+import types
+
+import pytest
+import torch
+
+from lestramanika_b200.pages import KVPages
+
+
+class FakeStream:
+    def __init__(self, handle, kind="stream"):
+        self.cuda_stream, self.kind, self.waits = handle, kind, 0
+
+    def synchronize(self):
+        self.waits += 1
+
+
+class FakeTorch:
+    """What KVPages asks of torch, on the CPU. ExternalStream of handle 0 is a stream of its own, as torch's is."""
+
+    def __init__(self):
+        self.default, self.now, self.scratch = FakeStream(0), FakeStream(11), []
+        self.uint8, self.int32, self.float32, self.bfloat16 = torch.uint8, torch.int32, torch.float32, torch.bfloat16
+        self.device = lambda *a: torch.device("cpu")
+        self._C = types.SimpleNamespace(_cuda_getCurrentRawStream=lambda d: self.now.cuda_stream)
+        self.cuda = types.SimpleNamespace(
+            current_stream=lambda d=None: self.now, default_stream=lambda d=None: self.default,
+            ExternalStream=lambda h, device=None: FakeStream(h or 99, "external"), Stream=FakeStream, stream=self._on,
+            is_current_stream_capturing=lambda: False)
+
+    class _On:
+        def __init__(self, t, s):
+            self.t, self.s = t, s
+
+        def __enter__(self):
+            self.was, self.t.now = self.t.now, self.s
+
+        def __exit__(self, *a):
+            self.t.now = self.was
+
+    def _on(self, s):
+        return self._On(self, s)
+
+    def empty(self, n, **kw):
+        self.scratch.append(self.now.cuda_stream)
+        return torch.empty(n, dtype=torch.uint8)
+
+    def zeros(self, *n, **kw):
+        kw.pop("device")
+        return torch.zeros(*n, **kw)
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    t = FakeTorch()
+    monkeypatch.setitem(__import__("sys").modules, "torch", t)
+    return t
+
+
+def _cache(**kw):
+    return KVPages(1, 4, 16, 2, 64, **kw)
+
+
+@pytest.mark.parametrize("given,handle", [(None, 11), (0, 0), (7, 7), (FakeStream(5), 5)])
+def test_scratch_belongs_to_the_call_s_stream(fake, given, handle):
+    cache = _cache()
+    cache._scratch(64, given)
+    assert fake.scratch == [handle]
+
+
+def test_sync_waits_for_the_stream_of_handle_0(fake):
+    cache = _cache()
+    cache.sync(0)
+    assert fake.default.waits == 1

@@ -23,7 +23,10 @@ PageBatch names the sequences of a call. PageSlots hands out the pages:
 
 Calls run on torch's current stream unless `stream` (a torch.cuda.Stream or
 a handle) says otherwise, and are asynchronous; sync() reports device-side
-errors.
+errors. A batch may be dropped at any time after the call; what its arrays
+hold is the caller's to keep until the call has run, and so are q, k, v and
+the outputs. A stream given as a handle has to outlive the batches that were
+used on it.
 """
 import ctypes
 
@@ -95,6 +98,7 @@ class PageBatch:
                               kv_len.data_ptr(), table.data_ptr(), table.shape[1])
         self._ref = ctypes.byref(self._c)
         self._ws = {}
+        self._tensors, self._streams = tensors, set()
 
 
 class KVPages:
@@ -187,8 +191,17 @@ class KVPages:
         if not 0 <= layer < self.n_layers or batch.device != self._dev:
             raise PickleError(ERR_ARG, "KVPages", "layer out of range, or a batch on another device")
         if stream is None:
-            return self._torch._C._cuda_getCurrentRawStream(self.device)
-        return stream if isinstance(stream, int) else stream.cuda_stream
+            st = self._torch._C._cuda_getCurrentRawStream(self.device)
+        else:
+            st = stream if isinstance(stream, int) else stream.cuda_stream
+        if st not in batch._streams:
+            # A batch is often dropped while its kernels still wait for their turn: its memory is not handed out before the
+            # streams that read it are through.
+            s = self._stream(stream)
+            for t in batch._tensors:
+                t.record_stream(s)
+            batch._streams.add(st)
+        return st
 
     def _run(self, fn, what, *args):
         if self._torch._C._cuda_getDevice() == self.device:

@@ -1,10 +1,11 @@
 """Streams of the paged KV cache's calls without a GPU: stand-ins for torch's streams record what would be done."""
+import sys
 import types
 
 import pytest
 import torch
 
-from lestramanika_b200.pages import KVPages
+from lestramanika_b200.pages import KVPages, PageBatch
 
 
 class FakeStream:
@@ -51,24 +52,40 @@ class FakeTorch:
 
 
 @pytest.fixture
-def fake(monkeypatch):
-    t = FakeTorch()
-    monkeypatch.setitem(__import__("sys").modules, "torch", t)
-    return t
+def fake():
+    return FakeTorch()
 
 
-def _cache(**kw):
-    return KVPages(1, 4, 16, 2, 64, **kw)
+def _cache(fake, monkeypatch):
+    with monkeypatch.context() as m:
+        m.setitem(sys.modules, "torch", fake)          # what the constructor imports and keeps
+        return KVPages(1, 4, 16, 2, 64)
 
 
 @pytest.mark.parametrize("given,handle", [(None, 11), (0, 0), (7, 7), (FakeStream(5), 5)])
-def test_scratch_belongs_to_the_call_s_stream(fake, given, handle):
-    cache = _cache()
+def test_scratch_belongs_to_the_call_s_stream(fake, monkeypatch, given, handle):
+    cache = _cache(fake, monkeypatch)
     cache._scratch(64, given)
     assert fake.scratch == [handle]
 
 
-def test_sync_waits_for_the_stream_of_handle_0(fake):
-    cache = _cache()
+def test_sync_waits_for_the_stream_of_handle_0(fake, monkeypatch):
+    cache = _cache(fake, monkeypatch)
     cache.sync(0)
     assert fake.default.waits == 1
+
+
+@pytest.mark.parametrize("given,handle", [(None, 11), (0, 0), (7, 7), (FakeStream(5), 5)])
+@pytest.mark.parametrize("starts", [False, True])
+def test_a_batch_outlives_the_streams_that_read_it(fake, monkeypatch, given, handle, starts):
+    seen = []
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: seen.append((t.data_ptr(), s.cuda_stream)))
+    kv, table, start = (torch.tensor(x, dtype=torch.int32) for x in ([3, 5], [[0, 1], [2, 3]], [0, 1, 2]))
+    batch = PageBatch(kv, table, q_start=start if starts else None)
+    cache = _cache(fake, monkeypatch)
+    for _ in range(2):
+        assert cache._call(batch, 0, given) == handle
+        assert cache._call(batch, 0, FakeStream(23)) == 23
+    want = [kv, table] + [start] * starts
+    for h in (handle, 23):
+        assert sorted(p for p, s in seen if s == h) == sorted(t.data_ptr() for t in want)

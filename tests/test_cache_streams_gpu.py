@@ -4,7 +4,7 @@ import torch
 
 import pages_ref as R
 from lestramanika_b200 import PickleError
-from lestramanika_b200.pages import KVPages, PageBatch
+from lestramanika_b200.pages import KVPages, PageBatch, PageSlots
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -31,3 +31,47 @@ def test_the_default_stream_as_a_handle():
         cache.attn_dev(0, short, q, out, stream=0)
         with pytest.raises(PickleError):
             cache.sync(0)
+
+
+@pytest.mark.parametrize("handle", ["stream", "raw", "current"])
+@pytest.mark.parametrize("prompt", [1, 20])
+def test_batches_dropped_while_a_side_stream_is_behind(handle, prompt):
+    """A serving loop on a stream that runs late: every step's batch is dropped at once, and the memory of the current stream
+    is written over meanwhile. The same as the loop without haste."""
+    HK, H, D, steps = 2, 8, 64, 24
+    g = torch.Generator().manual_seed(4)
+    rows = [[torch.randn((2 * prompt, n, D), generator=g).to(DEV) for n in (H, HK, HK)] for _ in range(steps)]
+
+    def loop(stream, late):
+        cache = KVPages(1, 80, 16, HK, D, rope_len=600)
+        slots = PageSlots(cache)
+        slots.admit("a")
+        slots.admit("b")
+        outs = []
+        torch.cuda.synchronize()
+        if late:
+            with torch.cuda.stream(stream):
+                torch.cuda._sleep(400_000_000)
+        for q, k, v in rows:
+            q, out = q.clone(), torch.empty_like(q)
+            torch.cuda.current_stream().synchronize()
+            batch = slots.batch(["a", "b"], [prompt, prompt])
+            if handle == "current":
+                with torch.cuda.stream(stream):
+                    slots.step(0, batch, q, k, v, out)
+            else:
+                slots.step(0, batch, q, k, v, out, stream=stream if handle == "stream" else stream.cuda_stream)
+            slots.advance(batch)
+            outs.append((q, out))
+            del batch
+            junk = [torch.full((n,), 3, dtype=torch.int32, device=DEV) for n in (2, 2, 3, 4, 8, 16, 32, 64)]
+            del junk
+        torch.cuda.synchronize()
+        cache.sync(stream)
+        return [o for _, o in outs], cache.pools[0].clone()
+
+    side = torch.cuda.Stream()
+    want, got = loop(side, False), loop(side, True)
+    assert torch.equal(want[1], got[1])
+    for a, b in zip(want[0], got[0]):
+        assert torch.equal(a, b)

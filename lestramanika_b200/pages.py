@@ -142,6 +142,9 @@ class KVPages:
         self.pools = list(pools)
         self.err = torch.zeros(1, dtype=torch.int32, device=dev)
         self._dev = dev
+        # The first call may be on another stream: what this one fills has to be there.
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(dev).synchronize()
         self._c = [PagesParams(p.data_ptr(), kv_type, n_pages, page_size, n_kv_heads, head_dim, self.err.data_ptr())
                    for p in self.pools]
         self._refs = [ctypes.byref(c) for c in self._c]

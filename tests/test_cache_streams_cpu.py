@@ -48,6 +48,7 @@ class FakeTorch:
 
     def zeros(self, *n, **kw):
         kw.pop("device")
+        self.filled = self.now.waits
         return torch.zeros(*n, **kw)
 
 
@@ -89,3 +90,8 @@ def test_a_batch_outlives_the_streams_that_read_it(fake, monkeypatch, given, han
     want = [kv, table] + [start] * starts
     for h in (handle, 23):
         assert sorted(p for p, s in seen if s == h) == sorted(t.data_ptr() for t in want)
+
+
+def test_a_new_cache_is_filled_before_any_stream_can_use_it(fake, monkeypatch):
+    _cache(fake, monkeypatch)
+    assert fake.now.waits == fake.filled + 1

@@ -75,3 +75,23 @@ def test_batches_dropped_while_a_side_stream_is_behind(handle, prompt):
     assert torch.equal(want[1], got[1])
     for a, b in zip(want[0], got[0]):
         assert torch.equal(a, b)
+
+
+def test_a_new_cache_on_a_stream_that_is_behind():
+    """The constructor's fill is over before a call on another stream writes rows."""
+    g = torch.Generator().manual_seed(6)
+    k, v = (torch.randn((40, 2, 64), generator=g).to(DEV) for _ in "kv")
+    ko, vo = torch.empty_like(k), torch.empty_like(v)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    cache = KVPages(0, 2000, 16, 2, 64)
+    kv, table = torch.tensor([40], dtype=torch.int32), torch.tensor([[5, 1900, 7]], dtype=torch.int32)
+    start = torch.tensor([0, 40], dtype=torch.int32)
+    with torch.cuda.stream(side):
+        batch = PageBatch(kv.to(DEV), table.to(DEV), q_start=start.to(DEV))
+    cache.append_dev(0, batch, k, v, stream=side)
+    torch.cuda.synchronize()
+    cache.read_dev(0, batch, ko, vo, stream=side)
+    cache.sync(side)
+    assert torch.equal(ko, k.bfloat16().float()) and torch.equal(vo, v.bfloat16().float())

@@ -25,10 +25,10 @@ Calls run on torch's current stream unless `stream` (a torch.cuda.Stream or
 a handle) says otherwise, and are asynchronous; sync() reports device-side
 errors. A batch may be dropped at any time after the call; what its arrays
 hold is the caller's to keep until the call has run, and so are q, k, v and
-the outputs. A stream given as a handle has to outlive the batches that were
-used on it.
+the outputs.
 """
 import ctypes
+import itertools
 
 import numpy as np
 
@@ -66,6 +66,9 @@ def _ints(t, what):
     return t
 
 
+_serials = itertools.count()
+
+
 class PageBatch:
     """The sequences of one call (pickle_cuda_batch_t).
 
@@ -98,7 +101,14 @@ class PageBatch:
                               kv_len.data_ptr(), table.data_ptr(), table.shape[1])
         self._ref = ctypes.byref(self._c)
         self._ws = {}
-        self._tensors, self._streams = tensors, set()
+        self._tensors, self._streams, self._serial = tensors, set(), next(_serials)
+
+
+class _Held:
+    """Arrays of the batches that the stream of a handle reads: `old` ones until the event, `young` ones after it."""
+
+    def __init__(self):
+        self.young, self.old, self.event = {}, {}, None
 
 
 class KVPages:
@@ -151,6 +161,7 @@ class KVPages:
         self._row_types = {torch.float32: ROW_F32, torch.bfloat16: ROW_BF16}
         self._lib = lib()
         self._layouts = {}
+        self._held = {}
 
     def _tables(self, rope_len, theta, inv_freq, dev):
         # src/pickle_fast.c:1638-1640, 1772-1788: half = min(D/2, 64), inv_freq and angles in F32.
@@ -197,14 +208,30 @@ class KVPages:
             st = self._torch._C._cuda_getCurrentRawStream(self.device)
         else:
             st = stream if isinstance(stream, int) else stream.cuda_stream
-        if st not in batch._streams:
-            # A batch is often dropped while its kernels still wait for their turn: its memory is not handed out before the
-            # streams that read it are through.
+        # A batch is often dropped while its kernels still wait for their turn: its memory is not handed out before the
+        # streams that read it are through. The allocator asks a stream that is marked when the memory is dropped, and
+        # the stream of a handle may be gone by then: what those read is held here.
+        if isinstance(stream, int) and stream:
+            self._hold(batch, stream)
+        elif st not in batch._streams:
             s = self._stream(stream)
             for t in batch._tensors:
                 t.record_stream(s)
             batch._streams.add(st)
         return st
+
+    def _hold(self, batch, handle):
+        held = self._held.get(handle)
+        if held is None:
+            held = self._held[handle] = _Held()
+        if len(held.young) >= 64 and batch._serial not in held.young:
+            cuda, s = self._torch.cuda, self._stream(handle)
+            captured = cuda.is_current_stream_capturing()
+            with cuda.stream(s):
+                captured = captured or cuda.is_current_stream_capturing()
+            if not captured and (held.event is None or held.event.query()):
+                held.old, held.young, held.event = held.young, {}, s.record_event()
+        held.young[batch._serial] = batch._tensors
 
     def _run(self, fn, what, *args):
         if self._torch._C._cuda_getDevice() == self.device:
@@ -309,6 +336,8 @@ class KVPages:
         """Wait for the stream's work and raise PICKLE_ERR_DEVICE for a device-side error recorded since the last."""
         torch = self._torch
         self._stream(stream).synchronize()
+        if isinstance(stream, int):
+            self._held.pop(stream, None)
         code = int(self.err.item())
         if code:
             self.err.zero_()

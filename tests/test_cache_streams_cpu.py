@@ -1,6 +1,7 @@
 """Streams of the paged KV cache's calls without a GPU: stand-ins for torch's streams record what would be done."""
 import sys
 import types
+import weakref
 
 import pytest
 import torch
@@ -9,8 +10,13 @@ from lestramanika_b200.pages import KVPages, PageBatch
 
 
 class FakeStream:
+    done = False                                       # whether events have come to pass
+
     def __init__(self, handle, kind="stream"):
         self.cuda_stream, self.kind, self.waits = handle, kind, 0
+
+    def record_event(self):
+        return types.SimpleNamespace(query=lambda: FakeStream.done)
 
     def synchronize(self):
         self.waits += 1
@@ -76,7 +82,7 @@ def test_sync_waits_for_the_stream_of_handle_0(fake, monkeypatch):
     assert fake.default.waits == 1
 
 
-@pytest.mark.parametrize("given,handle", [(None, 11), (0, 0), (7, 7), (FakeStream(5), 5)])
+@pytest.mark.parametrize("given,handle", [(None, 11), (0, 0), (FakeStream(5), 5)])
 @pytest.mark.parametrize("starts", [False, True])
 def test_a_batch_outlives_the_streams_that_read_it(fake, monkeypatch, given, handle, starts):
     seen = []
@@ -95,3 +101,33 @@ def test_a_batch_outlives_the_streams_that_read_it(fake, monkeypatch, given, han
 def test_a_new_cache_is_filled_before_any_stream_can_use_it(fake, monkeypatch):
     _cache(fake, monkeypatch)
     assert fake.now.waits == fake.filled + 1
+
+
+def test_what_the_stream_of_a_handle_reads_is_held(fake, monkeypatch):
+    """No stream that may be gone is asked: batches are held until an event behind their last call has come to pass."""
+    monkeypatch.setattr(torch.Tensor, "record_stream", None)
+    monkeypatch.setattr(FakeStream, "done", False)
+    cache, alive = _cache(fake, monkeypatch), []
+
+    def call(n, also=None):
+        for _ in range(n):
+            batch = PageBatch(torch.tensor([3], dtype=torch.int32), torch.tensor([[0]], dtype=torch.int32))
+            alive.append(weakref.ref(batch.kv_len))
+            for layer in range(2):
+                assert cache._call(batch, 0, 7) == 7
+            if also is not None:
+                cache._call(also, 0, 7)
+
+    kept = PageBatch(torch.tensor([4], dtype=torch.int32), torch.tensor([[0]], dtype=torch.int32))
+    mine = weakref.ref(kept.kv_len)
+    call(200, kept)
+    assert all(x() is not None for x in alive)
+    FakeStream.done = True
+    call(130, kept)
+    del kept                                           # its last call is not behind an event yet
+    assert mine() is not None
+    assert sum(x() is not None for x in alive) <= 3 * 64 and all(x() is not None for x in alive[-64:])
+    call(200)
+    assert mine() is None
+    cache.sync(7)
+    assert all(x() is None for x in alive)

@@ -23,9 +23,10 @@ PageBatch names the sequences of a call. PageSlots hands out the pages:
 
 Calls run on torch's current stream unless `stream` (a torch.cuda.Stream or
 a handle) says otherwise, and are asynchronous; sync() reports device-side
-errors. A batch may be dropped at any time after the call; what its arrays
-hold is the caller's to keep until the call has run, and so are q, k, v and
-the outputs.
+errors. A batch may be dropped at any time after the call, and a cache too,
+unless a stream was given as a handle: then after sync(handle). What the
+arrays hold is the caller's to keep until the call has run, and so are q, k, v
+and the outputs.
 """
 import ctypes
 import itertools
@@ -161,7 +162,8 @@ class KVPages:
         self._row_types = {torch.float32: ROW_F32, torch.bfloat16: ROW_BF16}
         self._lib = lib()
         self._layouts = {}
-        self._held = {}
+        self._held, self._streams = {}, set()
+        self._own = self.pools + [self.err] + list(rope or ())
 
     def _tables(self, rope_len, theta, inv_freq, dev):
         # src/pickle_fast.c:1638-1640, 1772-1788: half = min(D/2, 64), inv_freq and angles in F32.
@@ -213,11 +215,12 @@ class KVPages:
         # the stream of a handle may be gone by then: what those read is held here.
         if isinstance(stream, int) and stream:
             self._hold(batch, stream)
-        elif st not in batch._streams:
+        elif st not in batch._streams or st not in self._streams:
             s = self._stream(stream)
-            for t in batch._tensors:
+            for t in batch._tensors + self._own:
                 t.record_stream(s)
             batch._streams.add(st)
+            self._streams.add(st)
         return st
 
     def _hold(self, batch, handle):

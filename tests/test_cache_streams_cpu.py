@@ -94,8 +94,25 @@ def test_a_batch_outlives_the_streams_that_read_it(fake, monkeypatch, given, han
         assert cache._call(batch, 0, given) == handle
         assert cache._call(batch, 0, FakeStream(23)) == 23
     want = [kv, table] + [start] * starts
+    own = {t.data_ptr() for t in cache.pools + [cache.err]}
     for h in (handle, 23):
-        assert sorted(p for p, s in seen if s == h) == sorted(t.data_ptr() for t in want)
+        assert sorted(p for p, s in seen if s == h and p not in own) == sorted(t.data_ptr() for t in want)
+
+
+def test_a_cache_outlives_the_streams_that_use_it(fake, monkeypatch):
+    seen = []
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: seen.append((t.data_ptr(), s.cuda_stream)))
+    rope = torch.zeros(2, 40, 32)
+    with monkeypatch.context() as m:
+        m.setitem(sys.modules, "torch", fake)
+        cache = KVPages(1, 4, 16, 2, 64, n_layers=2, rope=(rope[0], rope[1]))
+    own = sorted(t.data_ptr() for t in (*cache.pools, cache.err, rope[0], rope[1]))
+    batch = PageBatch(torch.tensor([3], dtype=torch.int32), torch.tensor([[0]], dtype=torch.int32))
+    batch._streams.update((11, 5))                     # used with another cache before
+    cache._call(batch, 0, None)
+    cache._call(batch, 1, FakeStream(5))
+    for h in (11, 5):
+        assert sorted(p for p, s in seen if s == h and p in own) == own
 
 
 def test_a_new_cache_is_filled_before_any_stream_can_use_it(fake, monkeypatch):

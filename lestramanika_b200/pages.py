@@ -128,7 +128,8 @@ class KVPages:
         self._torch = torch
         self.kv_type, self.n_pages, self.page_size = kv_type, n_pages, page_size
         self.HK, self.D, self.n_layers, self.device = n_kv_heads, head_dim, n_layers, device
-        nbytes = pages_bytes(kv_type, n_pages, page_size, n_kv_heads, head_dim)
+        self._sizes = (kv_type, n_pages, page_size, n_kv_heads, head_dim, device)
+        nbytes = pages_bytes(*self._sizes[:5])
         if nbytes == 0 or n_layers < 1:
             raise PickleError(ERR_ARG, "KVPages", "page_size is a multiple of 16, head_dim 64 or 128")
         dev = torch.device("cuda", device)
@@ -296,7 +297,7 @@ class KVPages:
             raise PickleError(ERR_ARG, "KVPages", "window and sinks are not negative")
         if batch.n_tok == 0:
             return
-        key = (self, H, rt, window, sinks)
+        key = (self._sizes, H, rt, window, sinks)           # not the cache, which a kept batch would keep
         need = batch._ws.get(key)
         if need is None:
             need = batch._ws[key] = self.attn_workspace(batch, H, rt, window, sinks)

@@ -1,4 +1,7 @@
 """Streams of the paged KV cache's calls: whose memory is whose, and who waits for whom."""
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -95,3 +98,24 @@ def test_a_new_cache_on_a_stream_that_is_behind():
     cache.read_dev(0, batch, ko, vo, stream=side)
     cache.sync(side)
     assert torch.equal(ko, k.bfloat16().float()) and torch.equal(vo, v.bfloat16().float())
+
+
+def test_a_kept_batch_keeps_no_cache():
+    B = R.Batch("i8", 1, 128, 16, [4000], [1], 7)
+    kv, table, _ = B.tensors()
+    batch, q = PageBatch(kv, table), B.randn(1, 4, 128)
+    out, other = torch.empty_like(q), torch.empty_like(q)
+    cache = KVPages(1, B.n_pages, 16, 1, 128, pools=[B.pool])
+    cache.attn_dev(0, batch, q, out)
+    gone = weakref.ref(cache)
+    cache.sync()
+    del cache
+    gc.collect()
+    assert gone() is None
+    # another cache of the same sizes, and one of another type, whose call takes other pieces
+    KVPages(1, B.n_pages, 16, 1, 128, pools=[B.pool]).attn_dev(0, batch, q, other)
+    wide = R.Batch("bf16", 1, 128, 16, [4000], [1], 7)
+    assert torch.equal(wide.tensors()[1], table)
+    KVPages(0, wide.n_pages, 16, 1, 128, pools=[wide.pool]).attn_dev(0, batch, q, torch.empty_like(q))
+    torch.cuda.synchronize()
+    assert torch.equal(out, other)

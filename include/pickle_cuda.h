@@ -463,8 +463,9 @@ PICKLE_CUDA_API size_t pickle_cuda_pages_bytes(int kv_type, int n_pages, int pag
 /* Write the call's k, v rows (pre-RoPE, row_type) to their pages and give
  * the rotated q rows: NeoX half-split rotation of the first 2 * half
  * elements by row `position` of rope_sin / rope_cos [rope_len][half]
- * (half 0: no rotation, tables unused). The rotated k is rounded to F32
- * once, then quantised to the nearest code (ties to even). q and q_out may
+ * (half 0: no rotation, tables unused). The rotated k, and q where q_out is
+ * F32, are rounded to F32 once (BF16 q_out: twice, 2^-16 of its own
+ * rounding); k is then quantised to the nearest code (ties to even). q and q_out may
  * both be NULL; q_out may be q where the types agree. q [n_tok][n_heads][D],
  * k, v [n_tok][HK][D]; *_stride: elements between tokens (0: dense). Rows
  * are 16-byte aligned; half is a multiple of 8. Two rows of one call must

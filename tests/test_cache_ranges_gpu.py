@@ -99,3 +99,30 @@ def test_a_key_that_is_not_finite_among_the_largest(kv, call, pieces):
     cache.attn_dev(0, PageBatch(kv_len, table, q_start=start), q, out)
     cache.sync()
     assert torch.isnan(out[:q_len[0]]).all()
+
+
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+@pytest.mark.parametrize("D,half,H,HK", [(128, 64, 32, 8), (64, 32, 9, 3), (128, 16, 5, 1)])
+def test_rotated_q_is_rounded_once(rows, D, half, H, HK):
+    """To F32: half a step, 2^-24 of the value, and 2^-46 of the products' size for the errors' own sum. To BF16: half of
+    its step, 2^-8, from a sum whose two roundings are half an F32 step of the size each."""
+    B = R.Batch("i8", HK, D, 16, [400], [400], 61, fill=False)
+    kv, table, start = B.tensors()
+    ang = torch.rand((400, half), generator=torch.Generator().manual_seed(5), dtype=torch.float64) * 6.283185307179586
+    rope = ang.sin().float().to(DEV), ang.cos().float().to(DEV)
+    cache = KVPages(1, B.n_pages, 16, HK, D, pools=[B.pool], rope=rope)
+    batch = PageBatch(kv, table, q_start=start)
+    q, k = B.randn(400, H, D).to(R.ROWS[rows]), B.randn(400, HK, D).to(R.ROWS[rows])
+    wide, narrow = torch.empty((400, H, D), device=DEV), torch.empty((400, H, D), dtype=torch.bfloat16, device=DEV)
+    cache.append_dev(0, batch, k, k, q=q, q_out=wide)
+    cache.append_dev(0, batch, k, k, q=q, q_out=narrow)
+    cache.sync()
+    ref = R.rotate(q, *rope, half)
+    lo, hi = q[..., :half].double().abs(), q[..., half:2 * half].double().abs()
+    s, c = (x.double().abs()[:, None] for x in rope)
+    size = torch.cat([c * lo + s * hi, s * lo + c * hi, 0 * q[..., 2 * half:].double()], -1)
+    assert ((wide.double() - ref).abs() <= 2.0 ** -24 * ref.abs() + 2.0 ** -46 * size).all()
+    off = 2 * 2.0 ** -24 * size
+    assert ((narrow.double() - ref).abs() <= off + 2.0 ** -8 * (ref.abs() + off)).all()
+    if half < D // 2:                                  # and what is not rotated stays
+        assert torch.equal(wide[..., 2 * half:], q[..., 2 * half:].float())

@@ -415,9 +415,8 @@ PICKLE_CUDA_API int  pickle_cuda_generate_sampled(pickle_cuda_model_t* m, const 
  * covers 32 consecutive elements of a row and is the smallest power of two
  * for which every code is in range without clipping (2^-111 at least, so
  * blocks below about 2^-105 lose precision). A power of two makes every
- * element exactly a BF16 number: the tensor cores multiply the values the
- * cache stands for. A block with an element that is not finite gets scale
- * 255 and codes 0 and reads back as NaN. */
+ * element exactly a BF16 number. A block with an element that is not finite
+ * gets scale 255 and codes 0 and reads back as NaN. */
 #define PICKLE_CUDA_KV_BF16 0
 #define PICKLE_CUDA_KV_I8   1
 #define PICKLE_CUDA_KV_E4M3 2
@@ -487,9 +486,17 @@ PICKLE_CUDA_API int  pickle_cuda_pages_read_dev(const pickle_cuda_pages_t* pages
  * positions j <= p of a query at position p and, when window > 0, only those
  * with j > p - window or j < sinks. kv_head = h * HK / H, H / HK from 1 to 8.
  * q, out [n_tok][n_heads][D] of row_type (out may be q), accumulation in
- * F32. F32 rows keep F32 accuracy. With BF16 rows the softmax weights are
- * rounded to F16 (2^-12 of the weight) on 8-bit pages; on BF16 pages to BF16
- * (2^-9) where max_q * H / HK > 8 and to two BF16 numbers where it is not.
+ * F32. F32 rows keep F32 accuracy, on 8-bit pages within limits: their
+ * elements are multiplied as F16 numbers under a shared exponent, exact for
+ * blocks down to 2^-24 (int8) or 2^-15 (E4M3) of the largest scale, and off by
+ * up to 2^-24 of the largest magnitude below that. The largest is that of the k
+ * rows of the KV head (v: of the same 32 elements of its rows) that any row of
+ * the call sees in the sequence, so a row can lose bits to a key far larger
+ * than what it attends to. Softmax weights on 8-bit pages are right to 2^-32
+ * of the row's largest one. With BF16 rows the softmax weights are rounded to
+ * F16 (2^-12 of the weight) on 8-bit pages; on BF16 pages to BF16 (2^-9) where
+ * max_q * H / HK > 8 and to two BF16 numbers where it is not. Numbers of v
+ * above 2^90 may overflow in the sums.
  * Pages that no row of the call can see are never touched (their table
  * entries may be stale). A row that sees no key gives zeros. Keys on a page
  * outside the pool are left out and recorded in the error word. A k or v

@@ -20,8 +20,8 @@
 //               (which moves only when a score passes it by 2^8: the two
 //               warps of 32 rows vote, and only then read each other's half) and
 //               write P over S.
-// 8-bit codes become F16 numbers code * 2^(e - E), exact but for elements
-// 2^-24 below the reference: K has one E for 32 keys of a tile, which the
+// 8-bit codes become F16 numbers code * 2^(e - E), exact for e - E down to -24
+// (int8) or -15 (E4M3), see pages_decode.cuh: K has one E for 32 keys of a tile, which the
 // softmax undoes in the factor it applies anyway;
 // V has a running one per 32 elements, which a tile may pass by 2^5 (int8) or 2^7 (E4M3)
 // before it moves, and moving it rescales O. Elements keep the order that is cheapest to unpack;

@@ -14,8 +14,11 @@
 // chosen so that a lane's elements are contiguous.
 //
 // 8-bit codes become F16 numbers in registers: a code is exact in F16, and so
-// is code * 2^(e - E) for a reference exponent E near the largest one seen
-// (elements 2^-24 and more below it lose bits of no weight in the sums). K
+// is code * 2^(e - E) for a reference exponent E near the largest one seen, down
+// to e - E = -24 (int8) or -15 (E4M3). Smaller blocks are rounded to F16's smallest
+// step, 2^-24, and from e - E = -25 on count as 0: off by 2^-24 at most of the largest magnitude
+// that is behind E, which shows where a row sees, but gives next to no weight, a key far larger than
+// the others. K
 // has one E per warp, which the scores' factor undoes; V has one per 32
 // elements of the output, and moving it rescales O by a power of two. BF16
 // pages are multiplied as they are.
@@ -28,7 +31,8 @@
 //
 // The running maximum moves only when some score passes it by 2^8 (a warp
 // vote), so most cells need no reduction over the keys; p is held times 2^7
-// so that small weights stay above F16's subnormals.
+// so that small weights stay above F16's subnormals (one below 2^-21 of the largest
+// is off by 2^-32 of it at most).
 //
 // What bounds it: the instructions that turn codes into numbers (an SM streams
 // 39 GB/s of 8-bit cells with 16 warps, 5.7 TB/s in all, against 6.5 that HBM

@@ -111,6 +111,23 @@ def held_weights(k, v, pos, window, sinks):
     return (2.0 ** -32 * (see @ v.abs()))[:, None]
 
 
+def shared_exponents(q, k, v, mass):
+    """What blocks far below the largest ones add to the bound on 8-bit pages, [n][H][D] for q [n][H][D] over k, v
+    [HK][m][D], all of whose rows some row of the call sees.
+
+    A code is held as an F16 number under the exponent E of the largest scales: off by 2^-25 where the product is rounded to F16's
+    smallest step, by 448 2^-25 (E4M3) or 127 2^-25 (int8) where 2^(e - E) itself rounds to 0, in units in which the
+    largest magnitude is 232 or 63.75 at least (a scale is the smallest that holds it): 2^-24 of that magnitude. Of v it is the
+    largest of the same 32 elements of all rows; of k, of all rows, and a score is then off by the sum of |q_d|
+    times it over sqrt(D), which numerator and denominator both carry."""
+    n, H, D = q.shape
+    G = H // k.shape[0]
+    top_v = v.abs().unflatten(-1, (-1, 32)).amax((1, 3)).repeat_interleave(32, -1).repeat_interleave(G, 0)      # [H][D]
+    top_k = k.abs().amax((1, 2)).repeat_interleave(G, 0)                                                        # [H]
+    off = 2.0 ** -24 * q.double().abs().sum(-1) * top_k / math.sqrt(D)
+    return 2.0 ** -24 * top_v + 2 * off[..., None] * mass
+
+
 class Batch:
     """A random pool and ragged batch. Rows that no sequence owns are 255 bytes: NaN codes and NaN scales.
 

@@ -80,6 +80,70 @@ def test_magnitudes_that_differ_between_pieces(pattern, call, kv, rows, D, piece
         _check(B, G, rows, (B.randn(B.n_tok, G, D) * 2.0 ** -f).to(R.ROWS[rows]))
 
 
+@pytest.mark.parametrize("kv,rows,D,call", [x for x in FORMS if x[0] != "bf16"])
+@pytest.mark.parametrize("which", ["k", "v", "v first"])
+def test_a_key_far_larger_than_what_is_attended_to(which, kv, rows, D, call, monkeypatch):
+    """k: a block of one key is 2^f larger than all others, and q is next to 0 there. v: the same key's v is, and no row
+    gives it weight. The others lose 2^-24 of it at most, and nothing while they lie within 2^15 of it."""
+    monkeypatch.setenv("PICKLE_CUDA_PAGES_SPLITS", "1")
+    G, q_len = CALLS[call]
+    for f in (9, 13, 15, 17, 20, 23, 25, 30):
+        at = 0 if which == "v first" else 133
+
+        def amp(b, w, m):
+            x = torch.ones(m, D)
+            if m > at:
+                if which == "k" and w == 0:
+                    x[at, :32] = 2.0 ** f
+                elif which != "k" and w == 1:
+                    x[at] = 2.0 ** f
+                elif which != "k":
+                    x[at] = 0.0
+            return x
+
+        B = R.Batch(kv, 1, D, 16, [260, 37], q_len, 101 + f, amp=amp)
+        q = B.randn(B.n_tok, G, D)
+        if which == "k":
+            q[..., :32] *= 2.0 ** (-f - 12)
+        else:
+            # Every other key has a score near 40 or more: its weight is e^-40 of theirs.
+            kv_len, table, start = B.tensors()
+            cache = KVPages(R.KV[kv], B.n_pages, 16, 1, D, pools=[B.pool])
+            for b, m in enumerate(B.kv_len):
+                every = [j for j in range(m) if j != at]
+                B.k[b][:, every, 0] = 64.0
+            k = torch.cat([x[0] for x in B.k]).float().unsqueeze(1).contiguous()
+            v = torch.cat([x[0] for x in B.v]).float().unsqueeze(1).contiguous()
+            whole = torch.tensor([0] + [sum(B.kv_len[:i + 1]) for i in range(2)], dtype=torch.int32, device=DEV)
+            cache.append_dev(0, PageBatch(kv_len, table, q_start=whole), k, v)
+            ko, vo = torch.empty_like(k), torch.empty_like(v)
+            cache.read_dev(0, PageBatch(kv_len, table, q_start=whole), ko, vo)
+            cache.sync()
+            for b in range(2):
+                B.k[b] = ko[whole[b]:whole[b + 1], 0].double().unsqueeze(0)
+                B.v[b] = vo[whole[b]:whole[b + 1], 0].double().unsqueeze(0)
+            q[..., 0] = 40.0 * D ** 0.5 / 64.0
+        q = q.to(R.ROWS[rows])
+
+        def extra(b, mass):
+            if f <= 9:
+                return 0.0
+            t = B.start[b]
+            return R.shared_exponents(q[t:t + B.q_len[b]], B.k[b], B.v[b], mass)
+
+        _check(B, G, rows, q, extra)
+
+
+@pytest.mark.parametrize("kv,rows,D", [("i8", "f32", 128), ("i8", "bf16", 64), ("e4m3", "f32", 64), ("e4m3", "bf16", 128),
+                                       ("bf16", "f32", 128), ("bf16", "bf16", 64)])
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("k,v", [(60, 80), (-60, -80), (-60, 80), (0, 88)])
+def test_magnitudes_far_from_1(k, v, kv, rows, D, call):
+    G, q_len = CALLS[call]
+    B = R.Batch(kv, 1, D, 16, [260, 37], q_len, 111, amp=lambda b, which, m: 2.0 ** (v if which else k))
+    _check(B, G, rows, (B.randn(B.n_tok, G, D) * 2.0 ** -k).to(R.ROWS[rows]))
+
+
 @pytest.mark.parametrize("kv", ["i8", "e4m3"])
 @pytest.mark.parametrize("call", CALLS)
 def test_a_key_that_is_not_finite_among_the_largest(kv, call, pieces):

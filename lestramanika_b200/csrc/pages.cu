@@ -99,8 +99,9 @@ constexpr int ROW_WARPS = 4, ROW_AHEAD = 4;        // warps of a CTA; steps whos
 // A warp takes a token; its H + 2 HK rows are spread over gridDim.y warps. D / 8
 // lanes hold a row, 8 elements each, so a scale's 32 elements are 4 lanes and
 // a rotation partner is half / 8 lanes away. The token's sin / cos stay in
-// registers for all its rows. Bound by HBM: rows in, rotated q and codes out (4 ragged prompts
-// of up to 2048 tokens, 32 + 2 x 32 BF16 heads of 128, written as E4M3 and read back: 73 us for both, 3.9 TB/s);
+// registers for all its rows. Bound by its instructions, K's exact sums and the codes before all (4 ragged prompts
+// of up to 2048 tokens, 32 + 2 x 32 BF16 heads of 128, written as E4M3: 56 us with 68 % of the issue slots and 32 % of
+// DRAM's rate used; with the rows read back 73 us, 3.9 TB/s);
 // for one token a sequence by its launch (64 sequences, written and read back: 13 us for the two calls).
 // Finding a token's page takes four dependent loads, so a warp has many rows
 // to go with them (two tokens a warp, looked up together, were slower: 92 us
@@ -436,6 +437,9 @@ ChunkDims chunk_dims(int kv_type, int D, int row_type) {
 Plan plan_attn(const View& w, int kv_type, int D, int row_type, int H, int window, int sinks) {
     Plan p;
     const int G = H / w.HK;
+    // Up to 8 rows fit the few-rows kernel's one tile of columns. int8, 8 KV heads, the few-rows kernel and the other at 1
+    // to 8 rows: one sequence of 4096 keys 17 and 26 us, 16 of them 46 and 78, one of 32768 32 and 50, 16 of them 212 and
+    // 510. The other takes the same time up to 128 rows.
     p.few = (long long)w.max_q * G <= 8;
     const ChunkDims cd = p.few ? ChunkDims{CELL, 8} : chunk_dims(kv_type, D, row_type);
     p.blocks = (int)(((long long)w.max_q * G + cd.rows - 1) / cd.rows);

@@ -41,9 +41,10 @@
 // operands, tiles of 64 keys). Twins, 128 rows or fewer: 1.5 and 2.0. An item of 256 rows adds about 10 us
 // that nothing hides, one CTA filling an SM: page ids and q (3 us), the first
 // keys and softmax (5 us), the epilogue (3 us).
-// Measured (us): 2048 tokens on 8192, 32 / 8 heads, E4M3: 384 (806 TFLOP/s); 4 prompts of 2048, 32 / 32 heads,
-// BF16: 236 (583); 2 ragged ones up to 4001, window 1000, F32, D = 64, int8: 118;
+// Measured (us): 2048 tokens on 8192, 32 / 8 heads, E4M3: 383 (808 TFLOP/s); 4 prompts of 2048, 32 / 32 heads,
+// BF16: 236 to 243 (583 to 566, by GPU); 2 ragged ones up to 4001, window 1000, F32, D = 64, int8: 118;
 // 8 x 16 tokens on ragged contexts up to 4096, int8: 35.
+// Registers: 80 a softmax thread; 8-bit pages, D = 64 and F32 rows spill 196 bytes of them.
 //
 // Every wait is bounded; one that gives up records an error, and the CTA
 // lets its MMAs drain and frees its TMEM before it ends.

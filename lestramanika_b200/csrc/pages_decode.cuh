@@ -34,14 +34,17 @@
 // so that small weights stay above F16's subnormals (one below 2^-21 of the largest
 // is off by 2^-32 of it at most).
 //
-// What bounds it: the instructions that turn codes into numbers (an SM streams
-// 39 GB/s of 8-bit cells with 16 warps, 5.7 TB/s in all, against 6.5 that HBM
-// gives; BF16 cells 6.3 TB/s), then how evenly the SMs are filled: work comes in CTAs of one
-// piece of one sequence's keys, with about 5 us before and after its stream.
-// Measured (us; with the join): 16 sequences of 32768 keys, 64 / 8 heads, int8: 217 (5.1 TB/s); 64 ragged
-// ones up to 4096, 32 / 8 heads, E4M3, F32 rows: 88 (3.2); 16 with a window of
-// 4096 of 32768, BF16 pages, F32 rows: 48 (5.0); one of 4096, E4M3: 12.4 (latency: a launch, page
+// What bounds it: 8-bit cells, the chain of instructions that turns codes into numbers and products, at 16
+// warps an SM (an SM streams 39 GB/s of them at best, 5.7 TB/s in all, against 6.5 that HBM
+// gives and 6.3 of BF16 cells; 58 to 60 % of the issue slots are used, so it is latency as much as slots); then how
+// evenly the SMs are filled: work comes in CTAs of one
+// piece of one sequence's keys, with about 5 us before and after its stream. 64 ragged sequences keep an SM busy for 73 %
+// of the time on average.
+// Measured (us; with the join): 16 sequences of 32768 keys, 64 / 8 heads, int8: 217 to 231 (5.1 to 4.8 TB/s, by GPU);
+// 64 ragged ones up to 4096, 32 / 8 heads, E4M3, F32 rows: 88 (3.2); 16 with a window of
+// 4096 of 32768, BF16 pages, F32 rows: 48 (5.0); one of 4096, int8: 11.6 (latency: a launch, page
 // ids, keys, the join).
+// Registers: 128 a thread (168 with BF16 cells, D = 128, F32 rows), of which 16 to 48 bytes spill with F32 rows and D = 128.
 #pragma once
 #include <cuda_fp16.h>
 

@@ -1132,6 +1132,12 @@ def run_reference(args, rank):
     this arm's line at every N."""
     if rank != 0:
         return
+    import oracle
+    if not oracle.RefBlock.available():
+        # The C restatement that stands in elsewhere is not the reference.
+        print(json.dumps({"impl": "reference", "unavailable": "oracle/_ref/libref_attn_block.so, the reference's own "
+                          "attention block, is not built (its sources are not here)"}), flush=True)
+        return
     w = C4
     r = ref_decode(w, args.steps, args.warmup)
     out = {"impl": "reference", "metric": "decode-attn KV GB/s", "value": r["value"], "unit": "GB/s",

@@ -216,12 +216,13 @@ class KVPages:
         # the stream of a handle may be gone by then: what those read is held here.
         if isinstance(stream, int) and stream:
             self._hold(batch, stream)
-        elif st not in batch._streams or st not in self._streams:
-            s = self._stream(stream)
-            for t in batch._tensors + self._own:
-                t.record_stream(s)
-            batch._streams.add(st)
-            self._streams.add(st)
+            return st
+        for tensors, known in ((batch._tensors, batch._streams), (self._own, self._streams)):
+            if st not in known:
+                s = self._stream(stream)
+                for t in tensors:
+                    t.record_stream(s)
+                known.add(st)
         return st
 
     def _hold(self, batch, handle):

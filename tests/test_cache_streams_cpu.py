@@ -113,6 +113,10 @@ def test_a_cache_outlives_the_streams_that_use_it(fake, monkeypatch):
     cache._call(batch, 1, FakeStream(5))
     for h in (11, 5):
         assert sorted(p for p, s in seen if s == h and p in own) == own
+    # once: a new batch costs its own arrays, whatever the number of layers
+    before = len(seen)
+    cache._call(PageBatch(torch.tensor([3], dtype=torch.int32), torch.tensor([[0]], dtype=torch.int32)), 0, None)
+    assert len(seen) == before + 2
 
 
 def test_a_new_cache_is_filled_before_any_stream_can_use_it(fake, monkeypatch):
